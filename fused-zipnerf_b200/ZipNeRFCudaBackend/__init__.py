@@ -33,6 +33,14 @@ composite_and_resample = _C.composite_and_resample
 train_final = _C.train_final
 composite_final = _C.composite_final
 relu_backward_ = _C.relu_backward_  # addition: the ReLU backward + bias gradient of a bf16 layer (zf_mlp.h)
+# additions: the 8-bit row operators (zf_int8.h)
+quantize_rows = _C.quantize_rows
+dequantize_rows = _C.dequantize_rows
+rms_norm_int8 = _C.rms_norm_int8
+rms_norm_int8_backward = _C.rms_norm_int8_backward
+int8_linear = _C.int8_linear
+int8_weight_grad = _C.int8_weight_grad
+int8_status = _C.int8_status
 
 import sys as _sys  # noqa: E402
 
@@ -41,4 +49,5 @@ if str(_HERE.parent) not in _sys.path:  # zipnerf_b200 sits beside this package
 from zipnerf_b200.nerf_mlp import NerfMlp, nerf_mlp_parameters  # noqa: E402
 
 __all__ = ['grid_max_value', 'nerf_grid_grad_scale', 'Featurizer', 'set_rtc_dirs', 'Adam', 'generate_rays', 'view_rays', 'initialize_rays',
-           'sample_uniforms', 'composite_and_resample', 'train_final', 'composite_final', 'nerf_mlp_parameters', 'NerfMlp']
+           'sample_uniforms', 'composite_and_resample', 'train_final', 'composite_final', 'nerf_mlp_parameters', 'NerfMlp',
+           'quantize_rows', 'dequantize_rows', 'rms_norm_int8', 'rms_norm_int8_backward', 'int8_linear', 'int8_weight_grad', 'int8_status']

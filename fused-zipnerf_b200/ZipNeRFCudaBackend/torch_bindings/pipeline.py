@@ -16,5 +16,12 @@ sample_uniforms = _C.sample_uniforms
 composite_and_resample = _C.composite_and_resample
 train_final = _C.train_final
 composite_final = _C.composite_final
+quantize_rows = _C.quantize_rows
+dequantize_rows = _C.dequantize_rows
+rms_norm_int8 = _C.rms_norm_int8
+rms_norm_int8_backward = _C.rms_norm_int8_backward
+int8_linear = _C.int8_linear
+int8_weight_grad = _C.int8_weight_grad
+int8_status = _C.int8_status
 nerf_mlp_parameters = _backend.nerf_mlp_parameters
 NerfMlp = _backend.NerfMlp

@@ -4,7 +4,8 @@
 
 Outputs (next to the Python package that loads them, so they travel with the source tree):
   ZipNeRFCudaBackend/libzf_featurize.so  -- the sm_100a kernels and the C ABI of include/zf_featurize.h,
-                                            include/zf_sampling.h, include/zf_optim.h and include/zf_mlp.h
+                                            include/zf_sampling.h, include/zf_optim.h, include/zf_mlp.h and
+                                            include/zf_int8.h
   ZipNeRFCudaBackend/_C.<abi>.so         -- the PyTorch binding (ZipNeRFCudaBackend._C)
 
 Kernels are compiled ahead of time for sm_100a only (nvcc -gencode arch=compute_100a,code=sm_100a), one object per
@@ -34,6 +35,8 @@ NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '--use_fast_m
               '-Xcompiler', '-fPIC', '-Xcompiler', '-fvisibility=hidden', f'-I{INCLUDE}', f'-I{CSRC}']
 # extra nvcc flags for tuning builds (e.g. ZF_NVCC_EXTRA="-DZF_MIN_BLOCKS=6")
 NVCC_FLAGS += os.environ.get('ZF_NVCC_EXTRA', '').split()
+# the 8-bit row operators have no reference kernel to reproduce: IEEE quotients, subnormals kept
+PRECISE_FLAGS = [flag for flag in NVCC_FLAGS if flag != '--use_fast_math']
 
 
 def _headers() -> list[Path]:
@@ -72,13 +75,15 @@ def build_library(jobs: int | None = None, force: bool = False, subset: set | No
             if force or _stale(obj, [inst, *deps]):
                 steps.append([NVCC, *NVCC_FLAGS, f'-DZF_INST_F={features}', f'-DZF_INST_PAD={pad}', '-c', str(inst), '-o', str(obj)])
     # the C ABI translation units: featurizer objects, the sampling kernels, the Adam step, the MLP's ReLU backward, its
-    # tensor-core forward and backward, and its pack and unfold
+    # tensor-core forward and backward, and its pack and unfold; the 8-bit row operators
     abi_objects = []
-    for name in ['fz_capi', 'fz_sampling', 'fz_optim', 'fz_mlp', 'fz_nerf_mlp', 'fz_nerf_mlp_backward', 'fz_nerf_mlp_pack']:
+    for name in ['fz_capi', 'fz_sampling', 'fz_optim', 'fz_mlp', 'fz_nerf_mlp', 'fz_nerf_mlp_backward', 'fz_nerf_mlp_pack',
+                 'fz_int8_rows', 'fz_int8_linear', 'fz_int8_weight_grad']:
         source, obj = CSRC / f'{name}.cu', BUILD / f'{name}.o'
         abi_objects.append(obj)
         if force or _stale(obj, [source, *deps]):
-            steps.append([NVCC, *NVCC_FLAGS, '-c', str(source), '-o', str(obj)])
+            flags = PRECISE_FLAGS if name.startswith('fz_int8') else NVCC_FLAGS
+            steps.append([NVCC, *flags, '-c', str(source), '-o', str(obj)])
     # the largest instantiations first, so the parallel build ends evenly
     steps.sort(key=lambda cmd: -int(next((a.split('=')[1] for a in cmd if a.startswith('-DZF_INST_PAD=')), '999')))
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs or os.cpu_count() or 4) as pool:

@@ -1,5 +1,5 @@
 // torch_ext.cpp -- the PyTorch binding ZipNeRFCudaBackend._C over the C ABI (include/zf_featurize.h, zf_sampling.h,
-// zf_optim.h).
+// zf_optim.h, zf_int8.h).
 //
 // Mirrors the reference module (torch_bindings/bindings.cu:14-43) except its NeRF MLP: the attributes grid_max_value
 // and nerf_grid_grad_scale, set_rtc_dirs, the class Featurizer with its constructor, n_fp32_grad_rows, forward,
@@ -11,6 +11,7 @@
 // output, as in the reference. All computation happens in libzf_featurize.so; this file only converts tensors to
 // pointers and allocates the outputs the reference's wrappers return.
 #include "zf_featurize.h"
+#include "zf_int8.h"
 #include "zf_mlp.h"
 #include "zf_optim.h"
 #include "zf_sampling.h"
@@ -22,6 +23,7 @@
 
 #include <pybind11/stl.h>
 
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -621,6 +623,231 @@ private:
     zf_adam* m_adam = nullptr;
 };
 
+// ---------------------------------------------------------------------------------------------------------------------
+// int8 rows (zf_int8.h; no counterpart in the reference module): codes int8 [n, d] with a row stride that is a multiple
+// of 16, and one fp32 scale per row. The functions allocate their outputs; an operand left out is None.
+
+int row_type(const at::Tensor& tensor, const char* name) {
+    if (tensor.scalar_type() == at::kFloat) return ZF_FLOAT32;
+    if (tensor.scalar_type() == at::kBFloat16) return ZF_BFLOAT16;
+    throw std::runtime_error(std::string("ZipNeRF: ") + name + " must be float32 or bfloat16");
+}
+
+// the row stride of a 2D cuda tensor with unit column stride (a dimension of one row or column has any stride)
+int64_t row_stride(const at::Tensor& tensor, const char* name, const int64_t n, const int64_t d, const at::Device& device) {
+    if (!tensor.is_cuda() || tensor.dim() != 2 || tensor.size(0) != n || tensor.size(1) != d || (d > 1 && tensor.stride(1) != 1)) {
+        throw std::runtime_error(std::string("ZipNeRF: ") + name + " has an invalid layout");
+    }
+    if (tensor.device() != device) throw std::runtime_error(std::string("ZipNeRF: ") + name + " is on another device");
+    return n > 1 ? tensor.stride(0) : std::max<int64_t>(d, tensor.stride(0));
+}
+
+int64_t code_stride(const at::Tensor& codes, const char* name, const int64_t n, const int64_t d, const at::Device& device) {
+    if (codes.scalar_type() != at::kChar) throw std::runtime_error(std::string("ZipNeRF: ") + name + " must be int8");
+    const int64_t stride = row_stride(codes, name, n, d, device);
+    // the stride of a single row is never used
+    return n > 1 ? stride : (stride + 15) / 16 * 16;
+}
+
+void check_vector(const at::Tensor& tensor, const char* name, const int64_t n, const at::Device& device) {
+    check_input(tensor, name, at::kFloat);
+    if (tensor.dim() != 1 || tensor.size(0) != n) throw std::runtime_error(std::string("ZipNeRF: ") + name + " has the wrong size");
+    if (tensor.device() != device) throw std::runtime_error(std::string("ZipNeRF: ") + name + " is on another device");
+}
+
+void check_matrix(const at::Tensor& tensor, const char* name) {
+    if (!tensor.is_cuda() || tensor.dim() != 2 || tensor.size(1) == 0) throw std::runtime_error(std::string("ZipNeRF: ") + name + " must be a 2D cuda tensor");
+}
+
+at::Tensor empty_codes(const int64_t n, const int64_t d, const at::Tensor& like) {
+    return at::empty({n, (d + 15) / 16 * 16}, like.options().dtype(at::kChar)).narrow(1, 0, d);
+}
+
+int8_t* code_ptr(const at::Tensor& codes) { return static_cast<int8_t*>(codes.data_ptr()); }
+
+// the int32 that the tensor-core kernels of a device set to 1 if one of their bounded waits ran out
+at::Tensor int8_status(const at::Device& device) {
+    static std::vector<at::Tensor> status(static_cast<size_t>(c10::cuda::device_count()));
+    at::Tensor& t = status.at(static_cast<size_t>(device.index()));
+    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
+    return t;
+}
+
+at::ScalarType output_type(const at::ScalarType type) {
+    if (type != at::kFloat && type != at::kBFloat16) throw std::runtime_error("ZipNeRF: the output must be float32 or bfloat16");
+    return type;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, const bool power_of_two) {
+    check_matrix(x, "x");
+    const int64_t n = x.size(0), d = x.size(1);
+    zf_quantize_rows_args a{};
+    a.x = x.data_ptr();
+    a.x_dtype = row_type(x, "x");
+    a.x_stride = row_stride(x, "x", n, d, x.device());
+    a.n = n;
+    a.d = d;
+    a.power_of_two = power_of_two ? 1 : 0;
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor codes = empty_codes(n, d, x), scales = at::empty({n}, x.options().dtype(at::kFloat));
+    a.codes = code_ptr(codes);
+    a.codes_stride = (d + 15) / 16 * 16;
+    a.scales = scales.data_ptr<float>();
+    check_status(zf_quantize_rows(&a, current_stream()));
+    return {codes, scales};
+}
+
+at::Tensor dequantize_rows(const at::Tensor& codes, const at::Tensor& scales, const at::ScalarType dtype) {
+    check_matrix(codes, "codes");
+    const int64_t n = codes.size(0), d = codes.size(1);
+    zf_dequantize_rows_args a{};
+    a.codes_stride = code_stride(codes, "codes", n, d, codes.device());
+    check_vector(scales, "scales", n, codes.device());
+    const c10::cuda::CUDAGuard guard(codes.device());
+    at::Tensor out = at::empty({n, d}, codes.options().dtype(output_type(dtype)));
+    a.codes = code_ptr(codes);
+    a.scales = scales.data_ptr<float>();
+    a.n = n;
+    a.d = d;
+    a.out = out.data_ptr();
+    a.out_dtype = row_type(out, "output");
+    a.out_stride = d;
+    check_status(zf_dequantize_rows(&a, current_stream()));
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>, at::Tensor> rms_norm_int8(const at::Tensor& x, const std::optional<at::Tensor>& residual,
+                                                                                        const std::optional<at::Tensor>& weight, const double eps,
+                                                                                        const bool power_of_two) {
+    check_matrix(x, "x");
+    const int64_t n = x.size(0), d = x.size(1);
+    zf_rms_norm_int8_args a{};
+    a.x = x.data_ptr();
+    a.x_dtype = row_type(x, "x");
+    a.x_stride = row_stride(x, "x", n, d, x.device());
+    const c10::cuda::CUDAGuard guard(x.device());
+    std::optional<at::Tensor> sum;
+    if (residual.has_value()) {
+        a.residual = residual->data_ptr();
+        a.residual_dtype = row_type(*residual, "residual");
+        a.residual_stride = row_stride(*residual, "residual", n, d, x.device());
+        sum = at::empty({n, d}, residual->options());
+        a.sum = sum->data_ptr();
+        a.sum_stride = d;
+    }
+    if (weight.has_value()) {
+        check_vector(*weight, "weight", d, x.device());
+        a.weight = weight->data_ptr<float>();
+    }
+    a.n = n;
+    a.d = d;
+    a.eps = static_cast<float>(eps);
+    a.power_of_two = power_of_two ? 1 : 0;
+    at::Tensor codes = empty_codes(n, d, x), scales = at::empty({n}, x.options().dtype(at::kFloat)), rstd = at::empty({n}, scales.options());
+    a.codes = code_ptr(codes);
+    a.codes_stride = (d + 15) / 16 * 16;
+    a.scales = scales.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    check_status(zf_rms_norm_int8(&a, current_stream()));
+    return {codes, scales, sum, rstd};
+}
+
+at::Tensor rms_norm_int8_backward(const at::Tensor& grad, const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& rstd,
+                                  const std::optional<at::Tensor>& grad_residual) {
+    check_matrix(grad, "grad");
+    const int64_t n = grad.size(0), d = grad.size(1);
+    zf_rms_norm_int8_backward_args a{};
+    a.grad = grad.data_ptr();
+    a.grad_dtype = row_type(grad, "grad");
+    a.grad_stride = row_stride(grad, "grad", n, d, grad.device());
+    a.codes = code_ptr(codes);
+    a.codes_stride = code_stride(codes, "codes", n, d, grad.device());
+    check_vector(scales, "scales", n, grad.device());
+    check_vector(rstd, "rstd", n, grad.device());
+    a.scales = scales.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    if (grad_residual.has_value()) {
+        a.grad_residual = grad_residual->data_ptr();
+        a.grad_residual_dtype = row_type(*grad_residual, "grad_residual");
+        a.grad_residual_stride = row_stride(*grad_residual, "grad_residual", n, d, grad.device());
+    }
+    const c10::cuda::CUDAGuard guard(grad.device());
+    at::Tensor grad_x = at::empty({n, d}, grad_residual.has_value() ? grad_residual->options() : grad.options());
+    a.n = n;
+    a.d = d;
+    a.grad_x = grad_x.data_ptr();
+    a.grad_x_stride = d;
+    check_status(zf_rms_norm_int8_backward(&a, current_stream()));
+    return grad_x;
+}
+
+at::Tensor int8_linear(const at::Tensor& codes, const at::Tensor& scales, const at::Tensor& weight_codes, const at::Tensor& weight_scales,
+                       const std::optional<at::Tensor>& bias, const bool relu, const at::ScalarType dtype) {
+    check_matrix(codes, "codes");
+    check_matrix(weight_codes, "weight_codes");
+    const int64_t n = codes.size(0), in = codes.size(1), out = weight_codes.size(0);
+    const at::Device device = codes.device();
+    zf_int8_linear_args a{};
+    a.codes_stride = code_stride(codes, "codes", n, in, device);
+    a.weight_stride = code_stride(weight_codes, "weight_codes", out, in, device);
+    check_vector(scales, "scales", n, device);
+    check_vector(weight_scales, "weight_scales", out, device);
+    if (bias.has_value()) {
+        check_vector(*bias, "bias", out, device);
+        a.bias = bias->data_ptr<float>();
+    }
+    const c10::cuda::CUDAGuard guard(device);
+    at::Tensor output = at::empty({n, out}, codes.options().dtype(output_type(dtype)));
+    a.codes = code_ptr(codes);
+    a.scales = scales.data_ptr<float>();
+    a.weight_codes = code_ptr(weight_codes);
+    a.weight_scales = weight_scales.data_ptr<float>();
+    a.n = n;
+    a.in = in;
+    a.out = out;
+    a.relu = relu ? 1 : 0;
+    a.output = output.data_ptr();
+    a.output_dtype = row_type(output, "output");
+    a.output_stride = out;
+    a.status = int8_status(device).data_ptr<int>();
+    check_status(zf_int8_linear(&a, current_stream()));
+    return output;
+}
+
+void int8_weight_grad(const at::Tensor& grad, const at::Tensor& codes, const at::Tensor& scales, at::Tensor& grad_weight,
+                      const std::optional<at::Tensor>& grad_bias) {
+    check_matrix(grad, "grad");
+    check_matrix(codes, "codes");
+    const int64_t n = grad.size(0), out = grad.size(1), in = codes.size(1);
+    const at::Device device = grad.device();
+    if (grad.scalar_type() != at::kBFloat16) throw std::runtime_error("ZipNeRF: grad must be bfloat16");
+    zf_int8_weight_grad_args a{};
+    a.grad_stride = row_stride(grad, "grad", n, out, device);
+    a.codes_stride = code_stride(codes, "codes", n, in, device);
+    check_vector(scales, "scales", n, device);
+    check_input(grad_weight, "grad_weight", at::kFloat);
+    if (grad_weight.dim() != 2 || grad_weight.size(0) != out || grad_weight.size(1) != in || grad_weight.device() != device) {
+        throw std::runtime_error("ZipNeRF: grad_weight has the wrong size");
+    }
+    if (grad_bias.has_value()) {
+        check_vector(*grad_bias, "grad_bias", out, device);
+        a.grad_bias = grad_bias->data_ptr<float>();
+    }
+    const c10::cuda::CUDAGuard guard(device);
+    a.grad = reinterpret_cast<const uint16_t*>(grad.data_ptr());
+    a.codes = code_ptr(codes);
+    a.scales = scales.data_ptr<float>();
+    a.n = n;
+    a.in = in;
+    a.out = out;
+    a.grad_weight = grad_weight.data_ptr<float>();
+    a.workspace_bytes = zf_int8_weight_grad_workspace_size(n, in, out);
+    const at::Tensor workspace = at::empty({a.workspace_bytes}, grad.options().dtype(at::kByte));
+    a.workspace = workspace.data_ptr();
+    a.status = int8_status(device).data_ptr<int>();
+    check_status(zf_int8_weight_grad(&a, current_stream()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
@@ -650,4 +877,15 @@ PYBIND11_MODULE(_C, m) {
     m.def("train_final", &train_final);
     m.def("composite_final", &composite_final);
     m.def("relu_backward_", &relu_backward_);
+    using pybind11::arg;
+    m.def("quantize_rows", &quantize_rows, arg("x"), arg("power_of_two") = false);
+    m.def("dequantize_rows", &dequantize_rows, arg("codes"), arg("scales"), arg("dtype") = at::kBFloat16);
+    m.def("rms_norm_int8", &rms_norm_int8, arg("x"), arg("residual") = pybind11::none(), arg("weight") = pybind11::none(), arg("eps") = 1e-6,
+          arg("power_of_two") = false);
+    m.def("rms_norm_int8_backward", &rms_norm_int8_backward, arg("grad"), arg("codes"), arg("scales"), arg("rstd"),
+          arg("grad_residual") = pybind11::none());
+    m.def("int8_linear", &int8_linear, arg("codes"), arg("scales"), arg("weight_codes"), arg("weight_scales"), arg("bias") = pybind11::none(),
+          arg("relu") = false, arg("dtype") = at::kBFloat16);
+    m.def("int8_weight_grad", &int8_weight_grad, arg("grad"), arg("codes"), arg("scales"), arg("grad_weight"), arg("grad_bias") = pybind11::none());
+    m.def("int8_status", &int8_status, arg("device"));
 }

@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in include/zf_featurize.h, zf_sampling.h, zf_optim.h and zf_mlp.h (libzf_featurize.so).
+"""ctypes binding of the C ABI in include/zf_featurize.h, zf_sampling.h, zf_optim.h, zf_mlp.h and zf_int8.h
+(libzf_featurize.so).
 
 This is the binding a Python host without the PyTorch extension would write against the library. ``CFeaturizer``
 adds a thin convenience layer that takes PyTorch CUDA tensors and passes their device pointers; the computation
@@ -21,7 +22,9 @@ EXPORTED = ['zf_featurizer_create', 'zf_featurizer_destroy', 'zf_featurizer_n_ou
             'zf_direction_block_width', 'zf_initialize_rays', 'zf_view_rays', 'zf_generate_rays', 'zf_sample_uniforms',
             'zf_composite_and_resample', 'zf_train_final', 'zf_composite_final', 'zf_adam_create', 'zf_adam_destroy', 'zf_adam_step',
             'zf_adam_state', 'zf_relu_backward_bf16', 'zf_nerf_mlp_activations_size', 'zf_nerf_mlp_forward_tc', 'zf_nerf_mlp_backward_workspace_size',
-            'zf_nerf_mlp_backward_tc', 'zf_nerf_mlp_parameter_count', 'zf_nerf_mlp_pack', 'zf_nerf_mlp_unfold_grads']
+            'zf_nerf_mlp_backward_tc', 'zf_nerf_mlp_parameter_count', 'zf_nerf_mlp_pack', 'zf_nerf_mlp_unfold_grads', 'zf_quantize_rows',
+            'zf_dequantize_rows', 'zf_rms_norm_int8', 'zf_rms_norm_int8_backward', 'zf_int8_linear', 'zf_int8_weight_grad',
+            'zf_int8_weight_grad_workspace_size']
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -123,6 +126,42 @@ class zf_nerf_mlp_packed(ctypes.Structure):
     _fields_ = [(name, _p) for name in NERF_MLP_PACK_TARGETS]
 
 
+ZF_FLOAT32, ZF_BFLOAT16 = 0, 1
+
+
+class zf_quantize_rows_args(ctypes.Structure):
+    _fields_ = [('x', _p), ('x_dtype', ctypes.c_int), ('x_stride', _i64), ('n', _i64), ('d', _i64), ('power_of_two', ctypes.c_int), ('codes', _p),
+                ('codes_stride', _i64), ('scales', _p)]
+
+
+class zf_dequantize_rows_args(ctypes.Structure):
+    _fields_ = [('codes', _p), ('codes_stride', _i64), ('scales', _p), ('n', _i64), ('d', _i64), ('out', _p), ('out_dtype', ctypes.c_int),
+                ('out_stride', _i64)]
+
+
+class zf_rms_norm_int8_args(ctypes.Structure):
+    _fields_ = [('x', _p), ('x_dtype', ctypes.c_int), ('x_stride', _i64), ('residual', _p), ('residual_dtype', ctypes.c_int),
+                ('residual_stride', _i64), ('weight', _p), ('n', _i64), ('d', _i64), ('eps', ctypes.c_float), ('power_of_two', ctypes.c_int),
+                ('codes', _p), ('codes_stride', _i64), ('scales', _p), ('sum', _p), ('sum_stride', _i64), ('rstd', _p)]
+
+
+class zf_rms_norm_int8_backward_args(ctypes.Structure):
+    _fields_ = [('grad', _p), ('grad_dtype', ctypes.c_int), ('grad_stride', _i64), ('codes', _p), ('codes_stride', _i64), ('scales', _p),
+                ('rstd', _p), ('grad_residual', _p), ('grad_residual_dtype', ctypes.c_int), ('grad_residual_stride', _i64), ('n', _i64),
+                ('d', _i64), ('grad_x', _p), ('grad_x_stride', _i64)]
+
+
+class zf_int8_linear_args(ctypes.Structure):
+    _fields_ = [('codes', _p), ('codes_stride', _i64), ('scales', _p), ('weight_codes', _p), ('weight_stride', _i64), ('weight_scales', _p),
+                ('bias', _p), ('n', _i64), ('in_', _i64), ('out', _i64), ('relu', ctypes.c_int), ('output', _p), ('output_dtype', ctypes.c_int),
+                ('output_stride', _i64), ('status', _p)]
+
+
+class zf_int8_weight_grad_args(ctypes.Structure):
+    _fields_ = [('grad', _p), ('grad_stride', _i64), ('codes', _p), ('codes_stride', _i64), ('scales', _p), ('n', _i64), ('in_', _i64),
+                ('out', _i64), ('grad_weight', _p), ('grad_bias', _p), ('workspace', _p), ('workspace_bytes', _i64), ('status', _p)]
+
+
 class ZfError(RuntimeError):
     def __init__(self, code: int, message: str) -> None:
         super().__init__(message)
@@ -211,6 +250,12 @@ def load() -> ctypes.CDLL:
     lib.zf_nerf_mlp_pack.restype = ctypes.c_int
     lib.zf_nerf_mlp_unfold_grads.argtypes = [_p, _p, _p, _p]
     lib.zf_nerf_mlp_unfold_grads.restype = ctypes.c_int
+    # zf_int8.h
+    for name in ['zf_quantize_rows', 'zf_dequantize_rows', 'zf_rms_norm_int8', 'zf_rms_norm_int8_backward', 'zf_int8_linear', 'zf_int8_weight_grad']:
+        getattr(lib, name).argtypes = [ctypes.POINTER(globals()[name + '_args']), _p]
+        getattr(lib, name).restype = ctypes.c_int
+    lib.zf_int8_weight_grad_workspace_size.argtypes = [_i64, _i64, _i64]
+    lib.zf_int8_weight_grad_workspace_size.restype = _i64
     _lib = lib
     return lib
 
