@@ -1,78 +1,282 @@
 // fz_int8_linear.cu -- the linear layer on int8 rows (zf_int8_linear): output = scales x weight_scales x (codes
-// weight_codes^T) + bias, the integer products summed exactly.
+// weight_codes^T) + bias, the integer products summed exactly on the tcgen05 tensor cores (kind::i8, 32-bit
+// accumulators in tensor memory).
+//
+// A persistent kernel, one CTA per SM, walks over tiles of 128 rows x bn outputs (bn <= 256). Warp 0 (one lane) brings
+// 128-byte K-blocks of both operands into a ring by TMA tensor copies (128-byte swizzle, K-major, no multicast; columns
+// past `in` and rows past the operands arrive as zeros), warp 1 (one lane) issues the MMAs, warps 2-9 run the epilogue.
+// Tensor memory holds two accumulators, so the epilogue of a tile runs under the MMAs of the next. The epilogue turns an
+// accumulator's rows (one per lane) into output rows through a 128-byte-wide staging tile per warp, so that global
+// memory sees whole 128-byte pieces of rows.
+//
+// Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop; the CTA then
+// waits (bounded) for its own copies and MMAs in flight, frees its tensor memory and sets *status.
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_tcgen05.cuh"
+#include "fz_tma.cuh"
 
 #include <cuda_bf16.h>
-#include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 namespace zf::int8_linear {
 
-constexpr int kTile = 64;       // rows and outputs of a block
-constexpr int kDepth = 64;      // inputs per step
-constexpr int kBlock = 256;     // each thread: 4 x 4 outputs
+using namespace zf::nerf_mlp;  // the tcgen05 building blocks
+
+constexpr int kBlockK = 128;                 // bytes of K per ring stage: the swizzle's width
+constexpr int kMaxN = 256;                   // outputs of a tile at the most
+constexpr int kEpilogueWarps = 8;            // two groups of four warps; a group covers the 128 accumulator lanes
+constexpr int kFirstEpilogueWarp = 2;
+constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
+constexpr int kMaxStages = 8;
+constexpr int kOperandABytes = kTileRows * kBlockK;
+constexpr int kStagingBytes = 32 * 128;      // a warp's 32 rows x 128 bytes
+constexpr int kStagingOffset = 1024;         // behind the barriers
+constexpr int kRingOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
+constexpr int kMaxSmem = 227 * 1024;
+constexpr uint32_t kTmemColumns = 512;       // two accumulators of 256 columns
 
 struct Args {
-    const int8_t* codes;
-    int64_t codes_stride;
+    CUtensorMap x_map;       // codes [n, in], boxes of x_rows x 128
+    CUtensorMap w_map;       // weight codes [out, in], boxes of bn x 128
     const float* scales;
-    const int8_t* weight;
-    int64_t weight_stride;
     const float* weight_scales;
     const float* bias;
-    int64_t n, in, out;
+    int n, in, out;
+    int bn, x_rows;
+    int tiles_n;
+    int64_t tiles;
+    int stages, stage_bytes;
     bool relu;
+    bool vector;             // output rows on the 16-byte grid
     void* output;
     int64_t output_stride;
+    int* status;
 };
 
-// four codes at column k of a row (zeros past `in`)
-__device__ __forceinline__ int four_codes(const int8_t* row, const int64_t k, const int64_t in) {
-    if (k + 4 <= in) return *reinterpret_cast<const int*>(row + k);
-    uint32_t v = 0;
-    for (int e = 0; k + e < in; e++) v |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + e])) << (8 * e);
-    return static_cast<int>(v);
+// instruction descriptor of kind::i8: 32-bit integer accumulator (bits 4-5 = 2), signed 8-bit A and B (bits 7-9, 10-12 =
+// 1), both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
+__device__ __forceinline__ uint32_t int8_descriptor(const int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileRows >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_int8(const uint32_t d_tmem, const uint64_t a, const uint64_t b, const uint32_t idesc, const uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
 template <typename Out>
-__global__ void __launch_bounds__(kBlock) fz_int8_linear_kernel(const Args a) {
-    __shared__ int x[kTile][kDepth / 4 + 1];
-    __shared__ int w[kTile][kDepth / 4 + 1];
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile, out0 = static_cast<int64_t>(blockIdx.y) * kTile;
-    const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-    int sum[4][4] = {};
-    for (int64_t k0 = 0; k0 < a.in; k0 += kDepth) {
-        for (int i = threadIdx.x; i < kTile * kDepth / 4; i += kBlock) {
-            const int r = i / (kDepth / 4), c = i % (kDepth / 4);
-            x[r][c] = row0 + r < a.n ? four_codes(a.codes + (row0 + r) * a.codes_stride, k0 + 4 * c, a.in) : 0;
-            w[r][c] = out0 + r < a.out ? four_codes(a.weight + (out0 + r) * a.weight_stride, k0 + 4 * c, a.in) : 0;
+__device__ __forceinline__ uint32_t pack(const float lo, const float hi);
+template <>
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(const float lo, const float hi) { return pack_bf16x2(lo, hi); }
+
+template <typename Out>
+__global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __grid_constant__ Args a) {
+    constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));  // columns of a staging tile
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 512);
+    volatile int* abort = reinterpret_cast<volatile int*>(smem + 516);
+    const uint32_t bar0 = smem_address(bars);
+    auto full_bar = [&](const uint32_t i) { return bar0 + 8u * i; };
+    auto empty_bar = [&](const uint32_t i) { return bar0 + 8u * (kMaxStages + i); };
+    auto acc_full = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + i); };
+    auto acc_empty = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + 2 + i); };
+    const uint32_t drain_bar = bar0 + 8u * (2 * kMaxStages + 4);
+    const uint32_t ring = smem_address(smem) + kRingOffset;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int k_blocks = (a.in + kBlockK - 1) / kBlockK;
+    const uint32_t stages = static_cast<uint32_t>(a.stages);
+
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(kTmemColumns));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMaxStages; i++) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full_bar(i)), "r"(1));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty_bar(i)), "r"(1));
         }
-        __syncthreads();
-        for (int c = 0; c < kDepth / 4; c++) {
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                #pragma unroll
-                for (int j = 0; j < 4; j++) sum[i][j] = __dp4a(x[tr + 16 * i][c], w[tc + 16 * j][c], sum[i][j]);
+        for (int i = 0; i < 2; i++) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_full(i)), "r"(1));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty(i)), "r"(kEpilogueWarps));
+        }
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(drain_bar), "r"(1));
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *abort = 0;
+    }
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.x_map)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.w_map)) : "memory");
+            const uint32_t bytes = static_cast<uint32_t>((a.x_rows + a.bn) * kBlockK);
+            uint32_t stage = 0, round = 0;
+            bool ok = true;
+            for (int64_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
+                const int row = static_cast<int>(tile / a.tiles_n) * kTileRows, column = static_cast<int>(tile % a.tiles_n) * a.bn;
+                for (int k = 0; k < k_blocks; k++) {
+                    if (round > 0 && !(ok = wait_phase(empty_bar(stage), (round - 1) & 1u, abort))) break;
+                    const uint32_t at = ring + stage * a.stage_bytes;
+                    expect_bytes(full_bar(stage), bytes);
+                    tma_load_2d(at, &a.x_map, k * kBlockK, row, full_bar(stage));
+                    tma_load_2d(at + kOperandABytes, &a.w_map, k * kBlockK, column, full_bar(stage));
+                    if (++stage == stages) stage = 0, round++;
+                }
+            }
+            // every copy issued has landed before the CTA's shared memory can go to another CTA
+            for (uint32_t i = 0; i < stages; i++) {
+                const uint32_t issued = round + (i < stage ? 1 : 0);
+                if (issued > 0) drain_phase(full_bar(i), (issued - 1) & 1u);
             }
         }
-        __syncthreads();
     }
-    #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int64_t r = row0 + tr + 16 * i;
-        if (r >= a.n) continue;
-        #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int64_t o = out0 + tc + 16 * j;
-            if (o >= a.out) continue;
-            float v = static_cast<float>(sum[i][j]) * a.scales[r] * a.weight_scales[o];
-            if (a.bias != nullptr) v += a.bias[o];
-            if (a.relu && v < 0.0f) v = 0.0f;  // a comparison, so that a NaN stays one
-            static_cast<Out*>(a.output)[r * a.output_stride + o] = static_cast<Out>(v);
+    else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = int8_descriptor(a.bn);
+            uint32_t stage = 0, round = 0, count = 0;
+            bool ok = true;
+            for (int64_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, count++) {
+                const uint32_t buffer = count & 1u, use = count >> 1;
+                if (use > 0 && !wait_phase(acc_empty(buffer), (use - 1) & 1u, abort)) break;
+                fence_after_sync();
+                const uint32_t d = tmem + buffer * kMaxN;
+                for (int k = 0; k < k_blocks; k++) {
+                    if (!(ok = wait_phase(full_bar(stage), round & 1u, abort))) break;
+                    fence_after_sync();
+                    const uint32_t at = ring + stage * a.stage_bytes;
+                    const int steps = min(kBlockK, a.in - k * kBlockK);
+                    for (int s = 0; s < steps; s += 32) {
+                        // 8-row groups 1024 bytes apart; a K step is 32 bytes further along the swizzled rows
+                        mma_int8(d, smem_descriptor(at + s, 16, 1024, 2), smem_descriptor(at + kOperandABytes + s, 16, 1024, 2), idesc, k > 0 || s > 0);
+                    }
+                    commit(empty_bar(stage));
+                    if (++stage == stages) stage = 0, round++;
+                }
+                if (ok) commit(acc_full(buffer));
+            }
         }
     }
+    else {
+        const int group = (warp - kFirstEpilogueWarp) / 4, quadrant = warp % 4;
+        uint8_t* staging = smem + kStagingOffset + (warp - kFirstEpilogueWarp) * kStagingBytes;
+        uint32_t count = 0;
+        for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, count++) {
+            const uint32_t buffer = count & 1u, use = count >> 1;
+            const int row0 = static_cast<int>(tile / a.tiles_n) * kTileRows + 32 * quadrant, column0 = static_cast<int>(tile % a.tiles_n) * a.bn;
+            const int columns = min(a.bn, a.out - column0), rows = min(32, a.n - row0);
+            const float scale = lane < rows ? __ldg(a.scales + row0 + lane) : 0.0f;
+            // warp-uniform: the tensor-memory loads below are collective
+            if (!__all_sync(0xFFFFFFFFu, wait_phase(acc_full(buffer), use & 1u, abort))) break;
+            fence_after_sync();
+            const uint32_t acc = tmem + (static_cast<uint32_t>(32 * quadrant) << 16) + buffer * kMaxN;
+            for (int c = group * kChunk; c < columns && rows > 0; c += 2 * kChunk) {
+                #pragma unroll
+                for (int h = 0; h < kChunk; h += 32) {
+                    uint32_t r[32];
+                    issue_load<32>(acc + c + h, r);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    float v[32];
+                    #pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const int o = column0 + min(c + h + j, columns - 1);  // lanes past the columns repeat the last one
+                        float x = static_cast<float>(static_cast<int>(r[j])) * scale * __ldg(a.weight_scales + o);
+                        if (a.bias != nullptr) x += __ldg(a.bias + o);
+                        if (a.relu && x < 0.0f) x = 0.0f;  // a comparison, so that a NaN stays one
+                        v[j] = x;
+                    }
+                    // 16-byte piece p of row `lane` goes to place p ^ (lane & 7) of its 128 bytes: no bank conflicts
+                    constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
+                    #pragma unroll
+                    for (int j = 0; j < 32; j += kPer) {
+                        uint4 piece;
+                        if constexpr (sizeof(Out) == 4) {
+                            piece = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+                        }
+                        else {
+                            piece = make_uint4(pack<Out>(v[j], v[j + 1]), pack<Out>(v[j + 2], v[j + 3]), pack<Out>(v[j + 4], v[j + 5]),
+                                               pack<Out>(v[j + 6], v[j + 7]));
+                        }
+                        *reinterpret_cast<uint4*>(staging + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4)) = piece;
+                    }
+                }
+                __syncwarp();
+                Out* out = static_cast<Out*>(a.output) + static_cast<int64_t>(row0) * a.output_stride + column0 + c;
+                const int width = min(kChunk, columns - c);
+                if (a.vector) {
+                    #pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int r = 4 * i + lane / 8, p = lane % 8;
+                        constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
+                        const uint8_t* from = staging + r * 128 + ((p ^ (r & 7)) << 4);
+                        if (r < rows) {
+                            Out* to = out + r * a.output_stride + p * kPer;
+                            if ((p + 1) * kPer <= width) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                            else {
+                                for (int e = 0; p * kPer + e < width; e++) to[e] = reinterpret_cast<const Out*>(from)[e];
+                            }
+                        }
+                    }
+                }
+                else {
+                    for (int r = 0; r < rows; r++) {
+                        for (int e = lane; e < width; e += 32) {
+                            constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
+                            out[r * a.output_stride + e] = reinterpret_cast<const Out*>(staging + r * 128 + (((e / kPer) ^ (r & 7)) << 4))[e % kPer];
+                        }
+                    }
+                }
+                __syncwarp();
+            }
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(acc_empty(buffer));
+        }
+    }
+
+    // teardown: every role has left its loop; the MMAs already issued finish before the tensor memory is freed
+    fence_before_sync();
+    __syncthreads();
+    if (threadIdx.x == 32) {
+        commit(drain_bar);
+        drain_phase(drain_bar, 0);
+    }
+    if (threadIdx.x == 0 && *abort) atomicExch(a.status, kWaitTimeout);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+}
+
+// the tensor map of code rows [rows, columns], boxes of box_rows rows x 128 bytes with the 128-byte swizzle
+bool encode_codes(CUtensorMap* map, const int8_t* codes, const int64_t columns, const int64_t stride, const int64_t rows, const int box_rows) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = zf::tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(columns), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride)};
+    const cuuint32_t box[2] = {kBlockK, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t element_strides[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(codes), dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int round_up(const int v, const int to) { return (v + to - 1) / to * to; }
+
+template <typename Out>
+cudaError_t launch(Args& a, const unsigned blocks, cudaStream_t stream) {
+    const int smem = kRingOffset + a.stages * a.stage_bytes;
+    cudaError_t error = cudaFuncSetAttribute(fz_int8_linear_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    if (error != cudaSuccess) return error;
+    fz_int8_linear_kernel<Out><<<blocks, kThreads, smem, stream>>>(a);
+    return cudaGetLastError();
 }
 
 int invalid(const char* message) { return zf::set_error(ZF_ERROR_INVALID_ARGUMENT, message); }
@@ -98,12 +302,35 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
         || reinterpret_cast<uintptr_t>(args->output) % size != 0) {
         return invalid("int8_linear: invalid output");
     }
-    const Args a{args->codes, args->codes_stride, args->scales, args->weight_codes, args->weight_stride, args->weight_scales, args->bias,
-                 args->n, args->in, args->out, args->relu != 0, args->output, args->output_stride};
-    const dim3 grid(static_cast<unsigned>((a.n + kTile - 1) / kTile), static_cast<unsigned>((a.out + kTile - 1) / kTile));
-    if (grid.y > 65535) return invalid("int8_linear: invalid sizes");
-    if (args->output_dtype == ZF_FLOAT32) fz_int8_linear_kernel<float><<<grid, kBlock, 0, stream>>>(a);
-    else fz_int8_linear_kernel<__nv_bfloat16><<<grid, kBlock, 0, stream>>>(a);
-    const cudaError_t error = cudaGetLastError();
+    int device = 0, n_sms = 0;
+    cudaError_t error = cudaGetDevice(&device);
+    if (error == cudaSuccess) error = cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
+    if (error != cudaSuccess) return zf::set_cuda_error(error, "device query");
+    Args a{};
+    a.scales = args->scales;
+    a.weight_scales = args->weight_scales;
+    a.bias = args->bias;
+    a.n = static_cast<int>(args->n);
+    a.in = static_cast<int>(args->in);
+    a.out = static_cast<int>(args->out);
+    // the outputs in equal shares of at most 256, whole MMA columns of 16
+    const int shares = (a.out + kMaxN - 1) / kMaxN;
+    a.bn = round_up((a.out + shares - 1) / shares, 16);
+    a.x_rows = std::min(a.n, kTileRows);
+    a.tiles_n = (a.out + a.bn - 1) / a.bn;
+    a.tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * a.tiles_n;
+    a.stage_bytes = round_up(kOperandABytes + a.bn * kBlockK, 1024);
+    a.stages = std::min(kMaxStages, (kMaxSmem - kRingOffset) / a.stage_bytes);
+    a.relu = args->relu != 0;
+    a.vector = reinterpret_cast<uintptr_t>(args->output) % 16 == 0 && args->output_stride * size % 16 == 0;
+    a.output = args->output;
+    a.output_stride = args->output_stride;
+    a.status = args->status;
+    if (!encode_codes(&a.x_map, args->codes, args->in, args->codes_stride, args->n, a.x_rows)
+        || !encode_codes(&a.w_map, args->weight_codes, args->in, args->weight_stride, args->out, a.bn)) {
+        return zf::set_error(ZF_ERROR_CUDA, "int8_linear: no tensor map");
+    }
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(a.tiles, n_sms));
+    error = args->output_dtype == ZF_FLOAT32 ? launch<float>(a, blocks, stream) : launch<__nv_bfloat16>(a, blocks, stream);
     return error == cudaSuccess ? ZF_OK : zf::set_cuda_error(error, "int8_linear");
 }

@@ -19,9 +19,7 @@
 #include "zf_mlp.h"
 #include "fz_status.h"
 #include "fz_tcgen05.cuh"
-
-#include <cuda.h>
-#include <cudaTypedefs.h>
+#include "fz_tma.cuh"
 
 namespace zf::nerf_mlp {
 
@@ -432,12 +430,6 @@ struct WeightArgs {
     float* bias;                // bias[m] (+=), or null
 };
 
-__device__ __forceinline__ void tma_load_2d(const uint32_t dst, const CUtensorMap* map, const int x, const int y, const uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
-}
-
 __device__ __forceinline__ void red_add_v4(float* address, const float a, const float b, const float c, const float d) {
     asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(address), "f"(a), "f"(b), "f"(c), "f"(d) : "memory");
 }
@@ -604,17 +596,6 @@ __global__ void __launch_bounds__(kWgradThreads, 1) fz_nerf_mlp_backward_weight_
     __syncthreads();
     fence_after_sync();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-}
-
-// cuTensorMapEncodeTiled from the driver through the runtime (the library links no driver library)
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) p = nullptr;
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-    }();
-    return fn;
 }
 
 // the tensor map of a [n, cols] bf16 matrix with row stride `stride` elements, boxes of kKTile rows and 64 (128-byte
