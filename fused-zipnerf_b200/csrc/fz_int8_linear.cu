@@ -2,15 +2,18 @@
 // weight_codes^T) + bias, the integer products summed exactly on the tcgen05 tensor cores (kind::i8, 32-bit
 // accumulators in tensor memory).
 //
-// A persistent kernel, one CTA per SM, walks over tiles of 128 rows x bn outputs (bn <= 256). Warp 0 (one lane) brings
-// 128-byte K-blocks of both operands into a ring by TMA tensor copies (128-byte swizzle, K-major, no multicast; columns
-// past `in` and rows past the operands arrive as zeros), warp 1 (one lane) issues the MMAs, warps 2-9 run the epilogue.
-// Tensor memory holds two accumulators, so the epilogue of a tile runs under the MMAs of the next. The epilogue turns an
-// accumulator's rows (one per lane) into output rows through a 128-byte-wide staging tile per warp, so that global
-// memory sees whole 128-byte pieces of rows.
+// A persistent kernel walks over tiles of 128 rows x bn outputs (bn <= 256), one CTA per SM, or (kPair) of 256 rows, a
+// cluster of two CTAs per tile whose MMAs (cta_group::2) read both CTAs' shared memory: each CTA holds 128 rows and half
+// of the outputs' weights, so a tile's weights are fetched once for 256 rows. Warp 0 (one lane) brings 128-byte K-blocks
+// of both operands into a ring by TMA tensor copies (128-byte swizzle, K-major, no multicast; columns past `in` and rows
+// past the operands arrive as zeros), warp 1 (one lane, of the pair's first CTA) issues the MMAs, warps 2-9 run the
+// epilogue of the CTA's own 128 rows. Tensor memory holds two accumulators, so the epilogue of a tile runs under the MMAs
+// of the next. The epilogue turns an accumulator's rows (one per lane) into output rows through a 128-byte-wide staging
+// tile per warp, so that global memory sees whole 128-byte pieces of rows.
 //
-// Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop; the CTA then
-// waits (bounded) for its own copies and MMAs in flight, frees its tensor memory and sets *status.
+// Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop (the other CTA of
+// a pair runs out on its own); the CTA then waits (bounded) for its own copies and MMAs in flight, frees its tensor
+// memory and sets *status.
 #include "zf_int8.h"
 #include "fz_status.h"
 #include "fz_tcgen05.cuh"
@@ -33,23 +36,25 @@ constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
 constexpr int kMaxStages = 8;
 constexpr int kOperandABytes = kTileRows * kBlockK;
 constexpr int kStagingBytes = 32 * 128;      // a warp's 32 rows x 128 bytes
-constexpr int kStagingOffset = 1024;         // behind the barriers
+constexpr int kColumnsOffset = 1024;         // behind the barriers: per warp, a tile's weight scales and biases
+constexpr int kColumnsBytes = 2 * kMaxN * 4;
+constexpr int kStagingOffset = kColumnsOffset + kEpilogueWarps * kColumnsBytes;
 constexpr int kRingOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
 constexpr int kMaxSmem = 227 * 1024;
 constexpr uint32_t kTmemColumns = 512;       // two accumulators of 256 columns
+static_assert(kRingOffset % 1024 == 0, "the swizzled ring starts on a 1024-byte boundary");
 
 struct Args {
     CUtensorMap x_map;       // codes [n, in], boxes of x_rows x 128
-    CUtensorMap w_map;       // weight codes [out, in], boxes of bn x 128
+    CUtensorMap w_map;       // weight codes [out, in], boxes of w_rows x 128
     const float* scales;
     const float* weight_scales;
     const float* bias;
     int n, in, out;
-    int bn, x_rows;
+    int bn, x_rows, w_rows;  // outputs of a tile; operand rows that one CTA loads
     int tiles_n;
     int64_t tiles;
     int stages, stage_bytes;
-    bool relu;
     bool vector;             // output rows on the 16-byte grid
     void* output;
     int64_t output_stride;
@@ -58,25 +63,74 @@ struct Args {
 
 // instruction descriptor of kind::i8: 32-bit integer accumulator (bits 4-5 = 2), signed 8-bit A and B (bits 7-9, 10-12 =
 // 1), both K-major, N / 8 in bits 17-22, M / 16 in bits 24-28
-__device__ __forceinline__ uint32_t int8_descriptor(const int n) {
-    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTileRows >> 4) << 24);
+__device__ __forceinline__ uint32_t int8_descriptor(const int m, const int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+template <bool kPair>
 __device__ __forceinline__ void mma_int8(const uint32_t d_tmem, const uint64_t a, const uint64_t b, const uint32_t idesc, const uint32_t accumulate) {
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+    if constexpr (kPair) {
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+    }
+    else {
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+    }
 }
 
-template <typename Out>
-__device__ __forceinline__ uint32_t pack(const float lo, const float hi);
-template <>
-__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(const float lo, const float hi) { return pack_bf16x2(lo, hi); }
+// the MMAs issued so far arrive on the barrier when they are done; of a pair, on both CTAs' barriers at this offset
+template <bool kPair>
+__device__ __forceinline__ void commit_to(const uint32_t bar) {
+    if constexpr (kPair) {
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                     "h"(static_cast<uint16_t>(3))
+                     : "memory");
+    }
+    else commit(bar);
+}
 
-template <typename Out>
+// the address of the pair's first CTA's shared memory at this offset
+__device__ __forceinline__ uint32_t of_first_cta(const uint32_t address) {
+    uint32_t out;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(out) : "r"(address));
+    return out;
+}
+
+// an arrival on a barrier of the cluster; what it orders is tensor memory (fence_before_sync), so it does not wait for
+// this thread's global stores as a release at cluster scope would
+__device__ __forceinline__ void arrive_cluster(const uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// a copy of a pair: into this CTA's shared memory, counted on the first CTA's barrier
+__device__ __forceinline__ void tma_load_2d_pair(const uint32_t dst, const CUtensorMap* map, const int x, const int y, const uint32_t first_cta_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(first_cta_bar)
+                 : "memory");
+}
+
+__device__ __forceinline__ void sync_cluster() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// the larger of v and 0; a NaN stays one
+__device__ __forceinline__ float relu(const float v) {
+    float out;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(out) : "f"(v));
+    return out;
+}
+
+// kRelu: each output's ReLU, in the conversion for bf16
+template <typename Out, bool kRelu, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __grid_constant__ Args a) {
     constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));  // columns of a staging tile
+    constexpr int kPer = 16 / static_cast<int>(sizeof(Out));     // columns of 16 bytes
+    constexpr int kCtas = kPair ? 2 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + 512);
@@ -89,12 +143,20 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     const uint32_t drain_bar = bar0 + 8u * (2 * kMaxStages + 4);
     const uint32_t ring = smem_address(smem) + kRingOffset;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int rank = kPair ? blockIdx.x % 2 : 0;
+    const int64_t first_tile = blockIdx.x / kCtas, tile_step = gridDim.x / kCtas;
     const int k_blocks = (a.in + kBlockK - 1) / kBlockK;
     const uint32_t stages = static_cast<uint32_t>(a.stages);
 
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(kTmemColumns));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(kTmemColumns));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        }
+        else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_address(tmem_slot)), "r"(kTmemColumns));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
     }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
@@ -103,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
         }
         for (int i = 0; i < 2; i++) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_full(i)), "r"(1));
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty(i)), "r"(kEpilogueWarps));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty(i)), "r"(kCtas * kEpilogueWarps));
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(drain_bar), "r"(1));
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -111,6 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     }
     fence_before_sync();
     __syncthreads();
+    if constexpr (kPair) sync_cluster();  // the other CTA's barriers are ready for remote arrivals
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
@@ -118,33 +181,51 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
         if (lane == 0) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.x_map)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a.w_map)) : "memory");
-            const uint32_t bytes = static_cast<uint32_t>((a.x_rows + a.bn) * kBlockK);
+            const uint32_t bytes = static_cast<uint32_t>(kCtas * (a.x_rows + a.w_rows) * kBlockK);
             uint32_t stage = 0, round = 0;
             bool ok = true;
-            for (int64_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x) {
-                const int row = static_cast<int>(tile / a.tiles_n) * kTileRows, column = static_cast<int>(tile % a.tiles_n) * a.bn;
+            for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+                const int row = static_cast<int>(tile / a.tiles_n) * (kCtas * kTileRows) + rank * kTileRows;
+                const int column = static_cast<int>(tile % a.tiles_n) * a.bn + rank * a.w_rows;
                 for (int k = 0; k < k_blocks; k++) {
+                    // of a pair, the first CTA's MMAs have read the slot in both CTAs, so its barrier's last phase is over
                     if (round > 0 && !(ok = wait_phase(empty_bar(stage), (round - 1) & 1u, abort))) break;
                     const uint32_t at = ring + stage * a.stage_bytes;
-                    expect_bytes(full_bar(stage), bytes);
-                    tma_load_2d(at, &a.x_map, k * kBlockK, row, full_bar(stage));
-                    tma_load_2d(at + kOperandABytes, &a.w_map, k * kBlockK, column, full_bar(stage));
+                    if (rank == 0) expect_bytes(full_bar(stage), bytes);
+                    if constexpr (kPair) {
+                        const uint32_t bar = of_first_cta(full_bar(stage));
+                        tma_load_2d_pair(at, &a.x_map, k * kBlockK, row, bar);
+                        tma_load_2d_pair(at + kOperandABytes, &a.w_map, k * kBlockK, column, bar);
+                    }
+                    else {
+                        tma_load_2d(at, &a.x_map, k * kBlockK, row, full_bar(stage));
+                        tma_load_2d(at + kOperandABytes, &a.w_map, k * kBlockK, column, full_bar(stage));
+                    }
                     if (++stage == stages) stage = 0, round++;
                 }
             }
             // every copy issued has landed before the CTA's shared memory can go to another CTA
-            for (uint32_t i = 0; i < stages; i++) {
-                const uint32_t issued = round + (i < stage ? 1 : 0);
-                if (issued > 0) drain_phase(full_bar(i), (issued - 1) & 1u);
+            if (rank == 0) {
+                for (uint32_t i = 0; i < stages; i++) {
+                    const uint32_t issued = round + (i < stage ? 1 : 0);
+                    if (issued > 0) drain_phase(full_bar(i), (issued - 1) & 1u);
+                }
+            }
+            else if (!ok) {
+                // the first CTA may not have expected this CTA's last copies: they depend on nothing and land within
+                // microseconds (without an abort its drain above covers them)
+                const uint64_t start = global_ns();
+                while (global_ns() - start < 1000000) {
+                }
             }
         }
     }
     else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = int8_descriptor(a.bn);
+        if (lane == 0 && rank == 0) {
+            const uint32_t idesc = int8_descriptor(kCtas * kTileRows, a.bn);
             uint32_t stage = 0, round = 0, count = 0;
             bool ok = true;
-            for (int64_t tile = blockIdx.x; tile < a.tiles && ok; tile += gridDim.x, count++) {
+            for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, count++) {
                 const uint32_t buffer = count & 1u, use = count >> 1;
                 if (use > 0 && !wait_phase(acc_empty(buffer), (use - 1) & 1u, abort)) break;
                 fence_after_sync();
@@ -156,56 +237,78 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     const int steps = min(kBlockK, a.in - k * kBlockK);
                     for (int s = 0; s < steps; s += 32) {
                         // 8-row groups 1024 bytes apart; a K step is 32 bytes further along the swizzled rows
-                        mma_int8(d, smem_descriptor(at + s, 16, 1024, 2), smem_descriptor(at + kOperandABytes + s, 16, 1024, 2), idesc, k > 0 || s > 0);
+                        mma_int8<kPair>(d, smem_descriptor(at + s, 16, 1024, 2), smem_descriptor(at + kOperandABytes + s, 16, 1024, 2), idesc, k > 0 || s > 0);
                     }
-                    commit(empty_bar(stage));
+                    commit_to<kPair>(empty_bar(stage));
                     if (++stage == stages) stage = 0, round++;
                 }
-                if (ok) commit(acc_full(buffer));
+                if (ok) commit_to<kPair>(acc_full(buffer));
             }
         }
     }
     else {
         const int group = (warp - kFirstEpilogueWarp) / 4, quadrant = warp % 4;
         uint8_t* staging = smem + kStagingOffset + (warp - kFirstEpilogueWarp) * kStagingBytes;
+        float* columns_scale = reinterpret_cast<float*>(smem + kColumnsOffset + (warp - kFirstEpilogueWarp) * kColumnsBytes);
+        float* columns_bias = columns_scale + kMaxN;
         uint32_t count = 0;
-        for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x, count++) {
+        int columns_of = -1;  // the first output whose scales and biases are in shared memory
+        for (int64_t tile = first_tile; tile < a.tiles; tile += tile_step, count++) {
             const uint32_t buffer = count & 1u, use = count >> 1;
-            const int row0 = static_cast<int>(tile / a.tiles_n) * kTileRows + 32 * quadrant, column0 = static_cast<int>(tile % a.tiles_n) * a.bn;
+            const int row0 = static_cast<int>(tile / a.tiles_n) * (kCtas * kTileRows) + rank * kTileRows + 32 * quadrant;
+            const int column0 = static_cast<int>(tile % a.tiles_n) * a.bn;
             const int columns = min(a.bn, a.out - column0), rows = min(32, a.n - row0);
             const float scale = lane < rows ? __ldg(a.scales + row0 + lane) : 0.0f;
+            if (column0 != columns_of) {
+                for (int j = lane; j < kMaxN; j += 32) {
+                    columns_scale[j] = j < columns ? __ldg(a.weight_scales + column0 + j) : 0.0f;
+                    columns_bias[j] = j < columns && a.bias != nullptr ? __ldg(a.bias + column0 + j) : 0.0f;
+                }
+                __syncwarp();
+                columns_of = column0;
+            }
             // warp-uniform: the tensor-memory loads below are collective
             if (!__all_sync(0xFFFFFFFFu, wait_phase(acc_full(buffer), use & 1u, abort))) break;
             fence_after_sync();
             const uint32_t acc = tmem + (static_cast<uint32_t>(32 * quadrant) << 16) + buffer * kMaxN;
+            auto release = [&]() {
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (kPair) arrive_cluster(of_first_cta(acc_empty(buffer)));
+                    else arrive(acc_empty(buffer));
+                }
+            };
+            if (group * kChunk >= columns || rows <= 0) release();
             for (int c = group * kChunk; c < columns && rows > 0; c += 2 * kChunk) {
+                uint32_t acc_words[kChunk];
+                #pragma unroll
+                for (int h = 0; h < kChunk; h += 32) issue_load<32>(acc + c + h, acc_words + h);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if (c + 2 * kChunk >= columns) release();  // the accumulator is read: the next tile's MMAs may overwrite it
                 #pragma unroll
                 for (int h = 0; h < kChunk; h += 32) {
-                    uint32_t r[32];
-                    issue_load<32>(acc + c + h, r);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    float v[32];
-                    #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int o = column0 + min(c + h + j, columns - 1);  // lanes past the columns repeat the last one
-                        float x = static_cast<float>(static_cast<int>(r[j])) * scale * __ldg(a.weight_scales + o);
-                        if (a.bias != nullptr) x += __ldg(a.bias + o);
-                        if (a.relu && x < 0.0f) x = 0.0f;  // a comparison, so that a NaN stays one
-                        v[j] = x;
-                    }
+                    const uint32_t* r = acc_words + h;
                     // 16-byte piece p of row `lane` goes to place p ^ (lane & 7) of its 128 bytes: no bank conflicts
-                    constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
                     #pragma unroll
                     for (int j = 0; j < 32; j += kPer) {
-                        uint4 piece;
-                        if constexpr (sizeof(Out) == 4) {
-                            piece = make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3]));
+                        float v[kPer];
+                        #pragma unroll
+                        for (int e = 0; e < kPer; e += 4) {
+                            const float4 s = *reinterpret_cast<const float4*>(columns_scale + c + h + j + e);
+                            const float4 b = *reinterpret_cast<const float4*>(columns_bias + c + h + j + e);
+                            v[e] = fmaf(static_cast<float>(static_cast<int>(r[j + e])) * scale, s.x, b.x);
+                            v[e + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 1])) * scale, s.y, b.y);
+                            v[e + 2] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 2])) * scale, s.z, b.z);
+                            v[e + 3] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 3])) * scale, s.w, b.w);
                         }
-                        else {
-                            piece = make_uint4(pack<Out>(v[j], v[j + 1]), pack<Out>(v[j + 2], v[j + 3]), pack<Out>(v[j + 4], v[j + 5]),
-                                               pack<Out>(v[j + 6], v[j + 7]));
+                        uint32_t words[4];
+                        #pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            if constexpr (sizeof(Out) == 4) words[q] = __float_as_uint(kRelu ? relu(v[q]) : v[q]);
+                            else words[q] = kRelu ? pack_bf16x2_relu(v[2 * q], v[2 * q + 1]) : pack_bf16x2(v[2 * q], v[2 * q + 1]);
                         }
-                        *reinterpret_cast<uint4*>(staging + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4)) = piece;
+                        *reinterpret_cast<uint4*>(staging + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
                     }
                 }
                 __syncwarp();
@@ -215,7 +318,6 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int r = 4 * i + lane / 8, p = lane % 8;
-                        constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
                         const uint8_t* from = staging + r * 128 + ((p ^ (r & 7)) << 4);
                         if (r < rows) {
                             Out* to = out + r * a.output_stride + p * kPer;
@@ -229,31 +331,32 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                 else {
                     for (int r = 0; r < rows; r++) {
                         for (int e = lane; e < width; e += 32) {
-                            constexpr int kPer = 16 / static_cast<int>(sizeof(Out));
                             out[r * a.output_stride + e] = reinterpret_cast<const Out*>(staging + r * 128 + (((e / kPer) ^ (r & 7)) << 4))[e % kPer];
                         }
                     }
                 }
                 __syncwarp();
             }
-            fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(acc_empty(buffer));
         }
     }
 
     // teardown: every role has left its loop; the MMAs already issued finish before the tensor memory is freed
     fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 32) {
-        commit(drain_bar);
+    if (threadIdx.x == 32 && rank == 0) {
+        if constexpr (kPair) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar) : "memory");
+        else commit(drain_bar);
         drain_phase(drain_bar, 0);
     }
     if (threadIdx.x == 0 && *abort) atomicExch(a.status, kWaitTimeout);
     fence_before_sync();
     __syncthreads();
+    if constexpr (kPair) sync_cluster();  // no MMA, copy or arrival reaches this CTA any more
     fence_after_sync();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+    if (warp == 1) {
+        if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
+    }
 }
 
 // the tensor map of code rows [rows, columns], boxes of box_rows rows x 128 bytes with the 128-byte swizzle
@@ -270,13 +373,29 @@ bool encode_codes(CUtensorMap* map, const int8_t* codes, const int64_t columns, 
 
 int round_up(const int v, const int to) { return (v + to - 1) / to * to; }
 
-template <typename Out>
-cudaError_t launch(Args& a, const unsigned blocks, cudaStream_t stream) {
-    const int smem = kRingOffset + a.stages * a.stage_bytes;
-    cudaError_t error = cudaFuncSetAttribute(fz_int8_linear_kernel<Out>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+template <typename Out, bool kRelu, bool kPair>
+cudaError_t launch_kernel(const Args& a, const int n_sms, cudaStream_t stream) {
+    const auto kernel = fz_int8_linear_kernel<Out, kRelu, kPair>;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
     if (error != cudaSuccess) return error;
-    fz_int8_linear_kernel<Out><<<blocks, kThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    constexpr int kCtas = kPair ? 2 : 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(kCtas * static_cast<unsigned>(std::min<int64_t>(a.tiles, n_sms / kCtas)));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kRingOffset + a.stages * a.stage_bytes;
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = kCtas;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = kPair ? 1 : 0;
+    return cudaLaunchKernelEx(&config, kernel, a);
+}
+
+template <typename Out, bool kRelu>
+cudaError_t launch(const Args& a, const bool pair, const int n_sms, cudaStream_t stream) {
+    return pair ? launch_kernel<Out, kRelu, true>(a, n_sms, stream) : launch_kernel<Out, kRelu, false>(a, n_sms, stream);
 }
 
 int invalid(const char* message) { return zf::set_error(ZF_ERROR_INVALID_ARGUMENT, message); }
@@ -313,24 +432,28 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
     a.n = static_cast<int>(args->n);
     a.in = static_cast<int>(args->in);
     a.out = static_cast<int>(args->out);
-    // the outputs in equal shares of at most 256, whole MMA columns of 16
+    // more than one tile's rows: pairs of CTAs
+    const bool pair = a.n > kTileRows;
+    const int tile_rows = pair ? 2 * kTileRows : kTileRows;
+    // the outputs in equal shares of at most 256, whole MMA columns (16; of a pair 32)
     const int shares = (a.out + kMaxN - 1) / kMaxN;
-    a.bn = round_up((a.out + shares - 1) / shares, 16);
+    a.bn = round_up((a.out + shares - 1) / shares, pair ? 32 : 16);
     a.x_rows = std::min(a.n, kTileRows);
+    a.w_rows = pair ? a.bn / 2 : a.bn;
     a.tiles_n = (a.out + a.bn - 1) / a.bn;
-    a.tiles = static_cast<int64_t>((a.n + kTileRows - 1) / kTileRows) * a.tiles_n;
-    a.stage_bytes = round_up(kOperandABytes + a.bn * kBlockK, 1024);
+    a.tiles = static_cast<int64_t>((a.n + tile_rows - 1) / tile_rows) * a.tiles_n;
+    a.stage_bytes = round_up(kOperandABytes + a.w_rows * kBlockK, 1024);
     a.stages = std::min(kMaxStages, (kMaxSmem - kRingOffset) / a.stage_bytes);
-    a.relu = args->relu != 0;
     a.vector = reinterpret_cast<uintptr_t>(args->output) % 16 == 0 && args->output_stride * size % 16 == 0;
     a.output = args->output;
     a.output_stride = args->output_stride;
     a.status = args->status;
     if (!encode_codes(&a.x_map, args->codes, args->in, args->codes_stride, args->n, a.x_rows)
-        || !encode_codes(&a.w_map, args->weight_codes, args->in, args->weight_stride, args->out, a.bn)) {
+        || !encode_codes(&a.w_map, args->weight_codes, args->in, args->weight_stride, args->out, a.w_rows)) {
         return zf::set_error(ZF_ERROR_CUDA, "int8_linear: no tensor map");
     }
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(a.tiles, n_sms));
-    error = args->output_dtype == ZF_FLOAT32 ? launch<float>(a, blocks, stream) : launch<__nv_bfloat16>(a, blocks, stream);
+    const bool relu = args->relu != 0;
+    if (args->output_dtype == ZF_FLOAT32) error = relu ? launch<float, true>(a, pair, n_sms, stream) : launch<float, false>(a, pair, n_sms, stream);
+    else error = relu ? launch<__nv_bfloat16, true>(a, pair, n_sms, stream) : launch<__nv_bfloat16, false>(a, pair, n_sms, stream);
     return error == cudaSuccess ? ZF_OK : zf::set_cuda_error(error, "int8_linear");
 }
