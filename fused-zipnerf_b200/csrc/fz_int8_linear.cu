@@ -6,10 +6,15 @@
 // cluster of two CTAs per tile whose MMAs (cta_group::2) read both CTAs' shared memory: each CTA holds 128 rows and half
 // of the outputs' weights, so a tile's weights are fetched once for 256 rows. Warp 0 (one lane) brings 128-byte K-blocks
 // of both operands into a ring by TMA tensor copies (128-byte swizzle, K-major, no multicast; columns past `in` and rows
-// past the operands arrive as zeros), warp 1 (one lane, of the pair's first CTA) issues the MMAs, warps 2-9 run the
+// past the operands arrive as zeros), warp 1 (one lane, of the pair's first CTA) issues the MMAs, warps 2-17 run the
 // epilogue of the CTA's own 128 rows. Tensor memory holds two accumulators, so the epilogue of a tile runs under the MMAs
-// of the next. The epilogue turns an accumulator's rows (one per lane) into output rows through a 128-byte-wide staging
-// tile per warp, so that global memory sees whole 128-byte pieces of rows.
+// of the next.
+//
+// The epilogue reads accumulators in the 16x256b shape, in which a lane holds two neighbouring columns of every eight: the
+// weight scales and biases of its 16 columns stay in registers over the tiles of a column block. (With a row per lane
+// every column's scale and bias came from shared memory, and those reads were what bound the kernel.) bf16 rows go
+// through a staging tile per warp (stmatrix, 128-byte swizzle) and leave by TMA store when the output lies on the 16-byte
+// grid; fp32 pairs are stored as they are, 32-byte sectors at a time.
 //
 // Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop (the other CTA of
 // a pair runs out on its own); the CTA then waits (bounded) for its own copies and MMAs in flight, frees its tensor
@@ -30,15 +35,14 @@ using namespace zf::nerf_mlp;  // the tcgen05 building blocks
 
 constexpr int kBlockK = 128;                 // bytes of K per ring stage: the swizzle's width
 constexpr int kMaxN = 256;                   // outputs of a tile at the most
-constexpr int kEpilogueWarps = 8;            // two groups of four warps; a group covers the 128 accumulator lanes
+constexpr int kEpilogueWarps = 16;           // four groups of four warps; a group covers the 128 accumulator lanes
+constexpr int kGroups = kEpilogueWarps / 4;
 constexpr int kFirstEpilogueWarp = 2;
 constexpr int kThreads = 32 * (kFirstEpilogueWarp + kEpilogueWarps);
 constexpr int kMaxStages = 8;
 constexpr int kOperandABytes = kTileRows * kBlockK;
-constexpr int kStagingBytes = 32 * 128;      // a warp's 32 rows x 128 bytes
-constexpr int kColumnsOffset = 1024;         // behind the barriers: per warp, a tile's weight scales and biases
-constexpr int kColumnsBytes = 2 * kMaxN * 4;
-constexpr int kStagingOffset = kColumnsOffset + kEpilogueWarps * kColumnsBytes;
+constexpr int kStagingBytes = 32 * 128;      // a warp's 32 rows x 64 bf16 columns
+constexpr int kStagingOffset = 1024;         // behind the barriers
 constexpr int kRingOffset = kStagingOffset + kEpilogueWarps * kStagingBytes;
 constexpr int kMaxSmem = 227 * 1024;
 constexpr uint32_t kTmemColumns = 512;       // two accumulators of 256 columns
@@ -47,13 +51,14 @@ static_assert(kRingOffset % 1024 == 0, "the swizzled ring starts on a 1024-byte 
 struct Args {
     CUtensorMap x_map;       // codes [n, in], boxes of x_rows x 128
     CUtensorMap w_map;       // weight codes [out, in], boxes of w_rows x 128
+    CUtensorMap out_map;     // bf16 output [n, out], boxes of 32 x 64 (vector)
     const float* scales;
     const float* weight_scales;
     const float* bias;
     int n, in, out;
     int bn, x_rows, w_rows;  // outputs of a tile; operand rows that one CTA loads
     int tiles_n;
-    int64_t tiles;
+    int tiles;
     int stages, stage_bytes;
     bool vector;             // output rows on the 16-byte grid
     void* output;
@@ -118,6 +123,22 @@ __device__ __forceinline__ void sync_cluster() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// 16 accumulator lanes x 32 columns: of block i of 8 columns, words 4 i, 4 i + 1 are columns 2 (lane % 4), + 1 of row
+// lane / 4, words 4 i + 2, 4 i + 3 the same columns of row lane / 4 + 8 (no wait)
+__device__ __forceinline__ void load_16x256(const uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+// four 8 x 8 matrices of 16-bit elements; lane l gives the address of row l % 8 of matrix l / 8 and holds columns
+// 2 (l % 4), + 1 of row l / 4 of each
+__device__ __forceinline__ void store_matrices(const uint32_t address, const uint32_t m0, const uint32_t m1, const uint32_t m2, const uint32_t m3) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(address), "r"(m0), "r"(m1), "r"(m2), "r"(m3) : "memory");
+}
+
 // the larger of v and 0; a NaN stays one
 __device__ __forceinline__ float relu(const float v) {
     float out;
@@ -125,11 +146,25 @@ __device__ __forceinline__ float relu(const float v) {
     return out;
 }
 
+// the tiles of one CTA (or pair): every step-th one, outputs fastest, as tile rows m and tile columns c
+struct Walk {
+    int tile, m, c;
+    int step, step_m, step_c;
+
+    __device__ __forceinline__ Walk(const int first, const int step_, const int tiles_n)
+        : tile(first), m(first / tiles_n), c(first % tiles_n), step(step_), step_m(step_ / tiles_n), step_c(step_ % tiles_n) {}
+    __device__ __forceinline__ void next(const int tiles_n) {
+        tile += step;
+        m += step_m;
+        c += step_c;
+        if (c >= tiles_n) c -= tiles_n, m++;
+    }
+};
+
 // kRelu: each output's ReLU, in the conversion for bf16
 template <typename Out, bool kRelu, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __grid_constant__ Args a) {
-    constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));  // columns of a staging tile
-    constexpr int kPer = 16 / static_cast<int>(sizeof(Out));     // columns of 16 bytes
+    constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));  // neighbouring columns of one warp
     constexpr int kCtas = kPair ? 2 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
@@ -144,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     const uint32_t ring = smem_address(smem) + kRingOffset;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = kPair ? blockIdx.x % 2 : 0;
-    const int64_t first_tile = blockIdx.x / kCtas, tile_step = gridDim.x / kCtas;
+    const int first_tile = blockIdx.x / kCtas, tile_step = gridDim.x / kCtas;
     const int k_blocks = (a.in + kBlockK - 1) / kBlockK;
     const uint32_t stages = static_cast<uint32_t>(a.stages);
 
@@ -184,9 +219,8 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
             const uint32_t bytes = static_cast<uint32_t>(kCtas * (a.x_rows + a.w_rows) * kBlockK);
             uint32_t stage = 0, round = 0;
             bool ok = true;
-            for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-                const int row = static_cast<int>(tile / a.tiles_n) * (kCtas * kTileRows) + rank * kTileRows;
-                const int column = static_cast<int>(tile % a.tiles_n) * a.bn + rank * a.w_rows;
+            for (Walk walk(first_tile, tile_step, a.tiles_n); walk.tile < a.tiles && ok; walk.next(a.tiles_n)) {
+                const int row = walk.m * (kCtas * kTileRows) + rank * kTileRows, column = walk.c * a.bn + rank * a.w_rows;
                 for (int k = 0; k < k_blocks; k++) {
                     // of a pair, the first CTA's MMAs have read the slot in both CTAs, so its barrier's last phase is over
                     if (round > 0 && !(ok = wait_phase(empty_bar(stage), (round - 1) & 1u, abort))) break;
@@ -225,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
             const uint32_t idesc = int8_descriptor(kCtas * kTileRows, a.bn);
             uint32_t stage = 0, round = 0, count = 0;
             bool ok = true;
-            for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, count++) {
+            for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, count++) {
                 const uint32_t buffer = count & 1u, use = count >> 1;
                 if (use > 0 && !wait_phase(acc_empty(buffer), (use - 1) & 1u, abort)) break;
                 fence_after_sync();
@@ -249,29 +283,50 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     else {
         const int group = (warp - kFirstEpilogueWarp) / 4, quadrant = warp % 4;
         uint8_t* staging = smem + kStagingOffset + (warp - kFirstEpilogueWarp) * kStagingBytes;
-        float* columns_scale = reinterpret_cast<float*>(smem + kColumnsOffset + (warp - kFirstEpilogueWarp) * kColumnsBytes);
-        float* columns_bias = columns_scale + kMaxN;
+        const int pair_column = 2 * (lane % 4), lane_row = lane / 4;  // of every 8 columns; of every 8 rows
+        // weight scales and biases of this lane's columns: of block b of 8 columns, the chunk's for bf16 (8 blocks), the
+        // two chunks' for fp32 (4 blocks each)
+        float2 column_scale[8], column_bias[8];
+        auto block_column = [&](const int b) { return (b / (kChunk / 8) * kGroups + group) * kChunk + b % (kChunk / 8) * 8 + pair_column; };
+        int columns_of = -1;  // the first output of the tile whose scales and biases are held
+        // this lane's four rows of a tile row: 8 i + lane_row; the scales of the next tile's are fetched a tile ahead
+        auto row_of = [&](const int m) { return m * (kCtas * kTileRows) + rank * kTileRows + 32 * quadrant; };
+        auto fetch_scales = [&](const int m, float (&out)[4]) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = row_of(m) + 8 * i + lane_row;
+                out[i] = row < a.n ? __ldg(a.scales + row) : 0.0f;
+            }
+        };
         uint32_t count = 0;
-        int columns_of = -1;  // the first output whose scales and biases are in shared memory
-        for (int64_t tile = first_tile; tile < a.tiles; tile += tile_step, count++) {
+        float next_scales[4] = {};
+        Walk walk(first_tile, tile_step, a.tiles_n);
+        if (walk.tile < a.tiles) fetch_scales(walk.m, next_scales);
+        for (; walk.tile < a.tiles; count++) {
             const uint32_t buffer = count & 1u, use = count >> 1;
-            const int row0 = static_cast<int>(tile / a.tiles_n) * (kCtas * kTileRows) + rank * kTileRows + 32 * quadrant;
-            const int column0 = static_cast<int>(tile % a.tiles_n) * a.bn;
+            const int row0 = row_of(walk.m), column0 = walk.c * a.bn;
             const int columns = min(a.bn, a.out - column0), rows = min(32, a.n - row0);
-            const float scale = lane < rows ? __ldg(a.scales + row0 + lane) : 0.0f;
+            float scales[4];
+            #pragma unroll
+            for (int i = 0; i < 4; i++) scales[i] = next_scales[i];
+            walk.next(a.tiles_n);
+            if (walk.tile < a.tiles) fetch_scales(walk.m, next_scales);
             if (column0 != columns_of) {
-                for (int j = lane; j < kMaxN; j += 32) {
-                    columns_scale[j] = j < columns ? __ldg(a.weight_scales + column0 + j) : 0.0f;
-                    columns_bias[j] = j < columns && a.bias != nullptr ? __ldg(a.bias + column0 + j) : 0.0f;
+                #pragma unroll
+                for (int b = 0; b < 8; b++) {
+                    const int c = block_column(b);
+                    column_scale[b].x = c < columns ? __ldg(a.weight_scales + column0 + c) : 0.0f;
+                    column_scale[b].y = c + 1 < columns ? __ldg(a.weight_scales + column0 + c + 1) : 0.0f;
+                    column_bias[b].x = a.bias != nullptr && c < columns ? __ldg(a.bias + column0 + c) : 0.0f;
+                    column_bias[b].y = a.bias != nullptr && c + 1 < columns ? __ldg(a.bias + column0 + c + 1) : 0.0f;
                 }
-                __syncwarp();
                 columns_of = column0;
             }
             // warp-uniform: the tensor-memory loads below are collective
             if (!__all_sync(0xFFFFFFFFu, wait_phase(acc_full(buffer), use & 1u, abort))) break;
             fence_after_sync();
             const uint32_t acc = tmem + (static_cast<uint32_t>(32 * quadrant) << 16) + buffer * kMaxN;
-            auto release = [&]() {
+            auto release = [&]() {  // the accumulator is read: the next MMAs may overwrite it
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
@@ -279,65 +334,88 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     else arrive(acc_empty(buffer));
                 }
             };
-            if (group * kChunk >= columns || rows <= 0) release();
-            for (int c = group * kChunk; c < columns && rows > 0; c += 2 * kChunk) {
-                uint32_t acc_words[kChunk];
-                #pragma unroll
-                for (int h = 0; h < kChunk; h += 32) issue_load<32>(acc + c + h, acc_words + h);
-                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                if (c + 2 * kChunk >= columns) release();  // the accumulator is read: the next tile's MMAs may overwrite it
-                #pragma unroll
-                for (int h = 0; h < kChunk; h += 32) {
-                    const uint32_t* r = acc_words + h;
-                    // 16-byte piece p of row `lane` goes to place p ^ (lane & 7) of its 128 bytes: no bank conflicts
-                    #pragma unroll
-                    for (int j = 0; j < 32; j += kPer) {
-                        float v[kPer];
-                        #pragma unroll
-                        for (int e = 0; e < kPer; e += 4) {
-                            const float4 s = *reinterpret_cast<const float4*>(columns_scale + c + h + j + e);
-                            const float4 b = *reinterpret_cast<const float4*>(columns_bias + c + h + j + e);
-                            v[e] = fmaf(static_cast<float>(static_cast<int>(r[j + e])) * scale, s.x, b.x);
-                            v[e + 1] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 1])) * scale, s.y, b.y);
-                            v[e + 2] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 2])) * scale, s.z, b.z);
-                            v[e + 3] = fmaf(static_cast<float>(static_cast<int>(r[j + e + 3])) * scale, s.w, b.w);
-                        }
-                        uint32_t words[4];
-                        #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            if constexpr (sizeof(Out) == 4) words[q] = __float_as_uint(kRelu ? relu(v[q]) : v[q]);
-                            else words[q] = kRelu ? pack_bf16x2_relu(v[2 * q], v[2 * q + 1]) : pack_bf16x2(v[2 * q], v[2 * q + 1]);
-                        }
-                        *reinterpret_cast<uint4*>(staging + lane * 128 + ((((h + j) / kPer) ^ (lane & 7)) << 4)) = make_uint4(words[0], words[1], words[2], words[3]);
-                    }
-                }
+            const bool any = group * kChunk < columns && rows > 0;
+            if (!any) release();
+            if (sizeof(Out) == 2 && any) {
+                // the staging tile's last store has been read
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
-                Out* out = static_cast<Out*>(a.output) + static_cast<int64_t>(row0) * a.output_stride + column0 + c;
-                const int width = min(kChunk, columns - c);
-                if (a.vector) {
+            }
+            #pragma unroll
+            for (int i = 0; i < 64 / kChunk; i++) {
+                const int c = (i * kGroups + group) * kChunk;
+                if (c >= columns || rows <= 0) break;
+                const bool last = c + kGroups * kChunk >= columns;
+                #pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    uint32_t words[kChunk / 8][4];
                     #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int r = 4 * i + lane / 8, p = lane % 8;
-                        const uint8_t* from = staging + r * 128 + ((p ^ (r & 7)) << 4);
-                        if (r < rows) {
-                            Out* to = out + r * a.output_stride + p * kPer;
-                            if ((p + 1) * kPer <= width) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from);
+                    for (int b = 0; b < kChunk / 8; b += 4) load_16x256(acc + (static_cast<uint32_t>(16 * half) << 16) + c + 8 * b, &words[b][0]);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (last && half == 1) release();
+                    #pragma unroll
+                    for (int b = 0; b < kChunk / 8; b++) {
+                        #pragma unroll
+                        for (int e = 0; e < 4; e += 2) {  // rows 16 half + 8 (e / 2) + lane_row
+                            const float s = scales[2 * half + e / 2];
+                            const float2 w = column_scale[i * (kChunk / 8) + b], bias = column_bias[i * (kChunk / 8) + b];
+                            const float x = fmaf(static_cast<float>(static_cast<int>(words[b][e])) * s, w.x, bias.x);
+                            const float y = fmaf(static_cast<float>(static_cast<int>(words[b][e + 1])) * s, w.y, bias.y);
+                            if constexpr (sizeof(Out) == 2) words[b][e / 2] = kRelu ? pack_bf16x2_relu(x, y) : pack_bf16x2(x, y);
                             else {
-                                for (int e = 0; p * kPer + e < width; e++) to[e] = reinterpret_cast<const Out*>(from)[e];
+                                const float u = kRelu ? relu(x) : x, v = kRelu ? relu(y) : y;
+                                const int r = 16 * half + 4 * e + lane_row, at = c + 8 * b + pair_column;
+                                float* out = static_cast<float*>(a.output) + (row0 + r) * a.output_stride + column0 + at;
+                                if (r < rows) {
+                                    if (a.vector && at + 1 < columns) *reinterpret_cast<float2*>(out) = make_float2(u, v);
+                                    else {
+                                        if (at < columns) out[0] = u;
+                                        if (at + 1 < columns) out[1] = v;
+                                    }
+                                }
                             }
                         }
                     }
-                }
-                else {
-                    for (int r = 0; r < rows; r++) {
-                        for (int e = lane; e < width; e += 32) {
-                            out[r * a.output_stride + e] = reinterpret_cast<const Out*>(staging + r * 128 + (((e / kPer) ^ (r & 7)) << 4))[e % kPer];
+                    if constexpr (sizeof(Out) == 2) {
+                        // 8 x 8 matrices (block b, rows 0-7), (b, rows 8-15), (b + 1, ...): lane l holds the address of row
+                        // l % 8 of matrix l / 8; 16-byte piece p of row r lies at place p ^ (r & 7) of its 128 bytes
+                        const int r = 16 * half + lane % 16;
+                        #pragma unroll
+                        for (int b = 0; b < kChunk / 8; b += 2) {
+                            store_matrices(smem_address(staging) + r * 128 + (((b + lane / 16) ^ (r & 7)) << 4), words[b][0], words[b][1], words[b + 1][0],
+                                           words[b + 1][1]);
                         }
                     }
                 }
-                __syncwarp();
+            }
+            if (sizeof(Out) == 2 && any) {
+                const int c = group * kChunk;
+                if (a.vector) {
+                    fence_async_shared();
+                    __syncwarp();
+                    if (lane == 0) {
+                        // rows past n and columns past out are not written; bn is a multiple of 64 where a tile borders on another
+                        asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                         reinterpret_cast<uint64_t>(&a.out_map)),
+                                     "r"(column0 + c), "r"(row0), "r"(smem_address(staging))
+                                     : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                }
+                else {
+                    __syncwarp();
+                    const int width = min(kChunk, columns - c);
+                    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.output) + row0 * a.output_stride + column0 + c;
+                    for (int r = 0; r < rows; r++) {
+                        for (int e = lane; e < width; e += 32) {
+                            out[r * a.output_stride + e] = *reinterpret_cast<const __nv_bfloat16*>(staging + r * 128 + (((e / 8) ^ (r & 7)) << 4) + e % 8 * 2);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
         }
+        if (sizeof(Out) == 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     // teardown: every role has left its loop; the MMAs already issued finish before the tensor memory is freed
@@ -371,6 +449,18 @@ bool encode_codes(CUtensorMap* map, const int8_t* codes, const int64_t columns, 
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// the tensor map of the bf16 output [n, out], boxes of 32 rows x 64 columns with the 128-byte swizzle
+bool encode_output(CUtensorMap* map, void* output, const int64_t out, const int64_t stride, const int64_t n) {
+    const PFN_cuTensorMapEncodeTiled_v12000 encode = zf::tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(out), static_cast<cuuint64_t>(n)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
+    const cuuint32_t box[2] = {64, 32};
+    const cuuint32_t element_strides[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, output, dims, strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int round_up(const int v, const int to) { return (v + to - 1) / to * to; }
 
 template <typename Out, bool kRelu, bool kPair>
@@ -380,7 +470,7 @@ cudaError_t launch_kernel(const Args& a, const int n_sms, cudaStream_t stream) {
     if (error != cudaSuccess) return error;
     constexpr int kCtas = kPair ? 2 : 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(kCtas * static_cast<unsigned>(std::min<int64_t>(a.tiles, n_sms / kCtas)));
+    config.gridDim = dim3(kCtas * static_cast<unsigned>(std::min(a.tiles, n_sms / kCtas)));
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = kRingOffset + a.stages * a.stage_bytes;
     config.stream = stream;
@@ -435,13 +525,16 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
     // more than one tile's rows: pairs of CTAs
     const bool pair = a.n > kTileRows;
     const int tile_rows = pair ? 2 * kTileRows : kTileRows;
-    // the outputs in equal shares of at most 256, whole MMA columns (16; of a pair 32)
+    // the outputs in equal shares of at most 256: multiples of 32 for the MMAs, of 64 where a tile borders on another (the
+    // width of a bf16 store)
     const int shares = (a.out + kMaxN - 1) / kMaxN;
-    a.bn = round_up((a.out + shares - 1) / shares, pair ? 32 : 16);
+    a.bn = round_up((a.out + shares - 1) / shares, shares > 1 ? 64 : 32);
     a.x_rows = std::min(a.n, kTileRows);
     a.w_rows = pair ? a.bn / 2 : a.bn;
     a.tiles_n = (a.out + a.bn - 1) / a.bn;
-    a.tiles = static_cast<int64_t>((a.n + tile_rows - 1) / tile_rows) * a.tiles_n;
+    const int64_t tiles = static_cast<int64_t>((a.n + tile_rows - 1) / tile_rows) * a.tiles_n;
+    if (tiles > (1 << 30)) return invalid("int8_linear: invalid sizes");
+    a.tiles = static_cast<int>(tiles);
     a.stage_bytes = round_up(kOperandABytes + a.w_rows * kBlockK, 1024);
     a.stages = std::min(kMaxStages, (kMaxSmem - kRingOffset) / a.stage_bytes);
     a.vector = reinterpret_cast<uintptr_t>(args->output) % 16 == 0 && args->output_stride * size % 16 == 0;
@@ -450,6 +543,9 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
     a.status = args->status;
     if (!encode_codes(&a.x_map, args->codes, args->in, args->codes_stride, args->n, a.x_rows)
         || !encode_codes(&a.w_map, args->weight_codes, args->in, args->weight_stride, args->out, a.w_rows)) {
+        return zf::set_error(ZF_ERROR_CUDA, "int8_linear: no tensor map");
+    }
+    if (args->output_dtype == ZF_BFLOAT16 && a.vector && !encode_output(&a.out_map, args->output, args->out, args->output_stride, args->n)) {
         return zf::set_error(ZF_ERROR_CUDA, "int8_linear: no tensor map");
     }
     const bool relu = args->relu != 0;
