@@ -364,17 +364,34 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                             if constexpr (sizeof(Out) == 2) words[b][e / 2] = kRelu ? pack_bf16x2_relu(x, y) : pack_bf16x2(x, y);
                             else {
                                 const float u = kRelu ? relu(x) : x, v = kRelu ? relu(y) : y;
-                                const int r = 16 * half + 4 * e + lane_row, at = c + 8 * b + pair_column;
-                                float* out = static_cast<float*>(a.output) + (row0 + r) * a.output_stride + column0 + at;
-                                if (r < rows) {
-                                    if (a.vector && at + 1 < columns) *reinterpret_cast<float2*>(out) = make_float2(u, v);
-                                    else {
-                                        if (at < columns) out[0] = u;
-                                        if (at + 1 < columns) out[1] = v;
-                                    }
+                                const int r = 16 * half + 4 * e + lane_row, at = 8 * b + pair_column;
+                                if (a.vector && c + at + 1 < columns) {
+                                    float* out = static_cast<float*>(a.output) + (row0 + r) * a.output_stride + column0 + c + at;
+                                    if (r < rows) *reinterpret_cast<float2*>(out) = make_float2(u, v);
+                                }
+                                else {
+                                    // 16-byte piece p of row r at place p ^ (r & 7), as the bf16 rows
+                                    *reinterpret_cast<float2*>(staging + r * 128 + (((at / 4) ^ (r & 7)) << 4) + at % 4 * 4) = make_float2(u, v);
                                 }
                             }
                         }
+                    }
+                    if (sizeof(Out) == 4 && half == 1 && !(a.vector && c + kChunk <= columns)) {
+                        // rows off the 16-byte grid, or their last columns: 32 neighbouring columns of a row per store
+                        __syncwarp();
+                        const int first = a.vector ? (columns - c) & ~1 : 0;  // whole pairs are stored already
+                        float* out = static_cast<float*>(a.output) + row0 * a.output_stride + column0 + c;
+                        #pragma unroll
+                        for (int r = 0; r < 32; r += 8) {  // eight reads, then eight stores
+                            float held[8];
+                            #pragma unroll
+                            for (int e = 0; e < 8; e++) held[e] = *reinterpret_cast<const float*>(staging + (r + e) * 128 + (((lane / 4) ^ e) << 4) + lane % 4 * 4);
+                            #pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                if (r + e < rows && lane >= first && c + lane < columns) out[(r + e) * a.output_stride + lane] = held[e];
+                            }
+                        }
+                        __syncwarp();
                     }
                     if constexpr (sizeof(Out) == 2) {
                         // 8 x 8 matrices (block b, rows 0-7), (b, rows 8-15), (b + 1, ...): lane l holds the address of row
@@ -406,9 +423,19 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     __syncwarp();
                     const int width = min(kChunk, columns - c);
                     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.output) + row0 * a.output_stride + column0 + c;
-                    for (int r = 0; r < rows; r++) {
-                        for (int e = lane; e < width; e += 32) {
-                            out[r * a.output_stride + e] = *reinterpret_cast<const __nv_bfloat16*>(staging + r * 128 + (((e / 8) ^ (r & 7)) << 4) + e % 8 * 2);
+                    #pragma unroll
+                    for (int r = 0; r < 32; r += 8) {  // 32 neighbouring columns of a row per store; eight rows' reads, then their stores
+                        #pragma unroll
+                        for (int h = 0; h < kChunk; h += 32) {
+                            __nv_bfloat16 held[8];
+                            #pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                held[e] = *reinterpret_cast<const __nv_bfloat16*>(staging + (r + e) * 128 + ((((h + lane) / 8) ^ e) << 4) + lane % 8 * 2);
+                            }
+                            #pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                if (r + e < rows && h + lane < width) out[(r + e) * a.output_stride + h + lane] = held[e];
+                            }
                         }
                     }
                     __syncwarp();
@@ -435,6 +462,100 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
         if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemColumns));
     }
+}
+
+// A few rows (kRows at the most): bound by the weights' bytes and by latency, so no tiles: a warp takes kOutputs outputs,
+// its lanes 16 codes of each at a time, and multiplies them with the same codes of every row (dp4a, exact); one
+// integer reduction over the warp per output and row.
+constexpr int kFewBlock = 128;
+constexpr int kFewRows = 16;
+
+struct FewArgs {
+    const int8_t* codes;
+    int64_t codes_stride;
+    const float* scales;
+    const int8_t* weight;
+    int64_t weight_stride;
+    const float* weight_scales;
+    const float* bias;
+    int n, in, out;
+    bool relu;
+    void* output;
+    int64_t output_stride;
+};
+
+template <typename Out, int kRows, int kOutputs>
+__global__ void __launch_bounds__(kFewBlock) fz_int8_linear_few_kernel(const FewArgs a) {
+    const int lane = threadIdx.x % 32;
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * (kFewBlock / 32) + threadIdx.x / 32) * kOutputs;
+    if (first >= a.out) return;
+    const int outputs = static_cast<int>(min(static_cast<int64_t>(kOutputs), a.out - first));
+    int sums[kOutputs][kRows] = {};
+    // outputs and rows past the last repeat it: their sums are not used
+    const int8_t* w[kOutputs];
+    #pragma unroll
+    for (int o = 0; o < kOutputs; o++) w[o] = a.weight + (first + min(o, outputs - 1)) * a.weight_stride;
+    const int whole = a.in & ~15;
+    #pragma unroll 2
+    for (int k = 16 * lane; k < whole; k += 512) {
+        uint4 wv[kOutputs];
+        #pragma unroll
+        for (int o = 0; o < kOutputs; o++) wv[o] = __ldg(reinterpret_cast<const uint4*>(w[o] + k));
+        #pragma unroll
+        for (int r = 0; r < kRows; r++) {
+            const uint4 xv = __ldg(reinterpret_cast<const uint4*>(a.codes + min(r, a.n - 1) * a.codes_stride + k));
+            #pragma unroll
+            for (int o = 0; o < kOutputs; o++) {
+                int sum = __dp4a(static_cast<int>(xv.x), static_cast<int>(wv[o].x), sums[o][r]);
+                sum = __dp4a(static_cast<int>(xv.y), static_cast<int>(wv[o].y), sum);
+                sum = __dp4a(static_cast<int>(xv.z), static_cast<int>(wv[o].z), sum);
+                sums[o][r] = __dp4a(static_cast<int>(xv.w), static_cast<int>(wv[o].w), sum);
+            }
+        }
+    }
+    if (whole + lane < a.in) {  // the last codes, one per lane
+        #pragma unroll
+        for (int r = 0; r < kRows; r++) {
+            const int x = a.codes[min(r, a.n - 1) * a.codes_stride + whole + lane];
+            #pragma unroll
+            for (int o = 0; o < kOutputs; o++) sums[o][r] += x * w[o][whole + lane];
+        }
+    }
+    // lane l finishes sums l, l + 32, ... (row-major over rows and outputs)
+    constexpr int kSums = kOutputs * kRows;
+    #pragma unroll
+    for (int i = 0; i < kSums; i += 32) {
+        int mine = 0;
+        #pragma unroll
+        for (int j = i; j < kSums && j < i + 32; j++) {
+            const int sum = __reduce_add_sync(0xFFFFFFFFu, sums[j % kOutputs][j / kOutputs]);
+            if (lane == j - i) mine = sum;
+        }
+        const int r = (i + lane) / kOutputs, o = (i + lane) % kOutputs;
+        if (i + lane < kSums && r < a.n && o < outputs) {
+            const float s = __ldg(a.scales + r), ws = __ldg(a.weight_scales + first + o);
+            float v = fmaf(static_cast<float>(mine) * s, ws, a.bias != nullptr ? __ldg(a.bias + first + o) : 0.0f);
+            if (a.relu) v = relu(v);
+            static_cast<Out*>(a.output)[r * a.output_stride + first + o] = static_cast<Out>(v);
+        }
+    }
+}
+
+template <typename Out>
+cudaError_t launch_few(const FewArgs& a, cudaStream_t stream) {
+    auto run = [&](auto rows, auto outputs) {
+        constexpr int kRows = decltype(rows)::value, kOutputs = decltype(outputs)::value;
+        constexpr int kPerBlock = kFewBlock / 32 * kOutputs;
+        const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(a.out) + kPerBlock - 1) / kPerBlock);
+        fz_int8_linear_few_kernel<Out, kRows, kOutputs><<<blocks, kFewBlock, 0, stream>>>(a);
+    };
+    using std::integral_constant;
+    if (a.n == 1) run(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    else if (a.n == 2) run(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    else if (a.n <= 4) run(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (a.n <= 8) run(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else run(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    return cudaGetLastError();
 }
 
 // the tensor map of code rows [rows, columns], boxes of box_rows rows x 128 bytes with the 128-byte swizzle
@@ -511,8 +632,15 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
         || reinterpret_cast<uintptr_t>(args->output) % size != 0) {
         return invalid("int8_linear: invalid output");
     }
+    cudaError_t error;
+    if (args->n <= kFewRows) {
+        const FewArgs f{args->codes, args->codes_stride, args->scales, args->weight_codes, args->weight_stride, args->weight_scales, args->bias,
+                        static_cast<int>(args->n), static_cast<int>(args->in), static_cast<int>(args->out), args->relu != 0, args->output, args->output_stride};
+        error = args->output_dtype == ZF_FLOAT32 ? launch_few<float>(f, stream) : launch_few<__nv_bfloat16>(f, stream);
+        return error == cudaSuccess ? ZF_OK : zf::set_cuda_error(error, "int8_linear");
+    }
     int device = 0, n_sms = 0;
-    cudaError_t error = cudaGetDevice(&device);
+    error = cudaGetDevice(&device);
     if (error == cudaSuccess) error = cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
     if (error != cudaSuccess) return zf::set_cuda_error(error, "device query");
     Args a{};
@@ -526,13 +654,15 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
     const bool pair = a.n > kTileRows;
     const int tile_rows = pair ? 2 * kTileRows : kTileRows;
     // the outputs in equal shares of at most 256: multiples of 32 for the MMAs, of 64 where a tile borders on another (the
-    // width of a bf16 store)
-    const int shares = (a.out + kMaxN - 1) / kMaxN;
+    // width of a bf16 store); halved while twice the tiles still find a multiprocessor each
+    const int64_t tiles_m = (a.n + tile_rows - 1) / tile_rows;
+    int shares = (a.out + kMaxN - 1) / kMaxN;
+    while (tiles_m * shares * 2 <= (pair ? n_sms / 2 : n_sms) && a.out > 64 * shares) shares *= 2;
     a.bn = round_up((a.out + shares - 1) / shares, shares > 1 ? 64 : 32);
     a.x_rows = std::min(a.n, kTileRows);
     a.w_rows = pair ? a.bn / 2 : a.bn;
     a.tiles_n = (a.out + a.bn - 1) / a.bn;
-    const int64_t tiles = static_cast<int64_t>((a.n + tile_rows - 1) / tile_rows) * a.tiles_n;
+    const int64_t tiles = tiles_m * a.tiles_n;
     if (tiles > (1 << 30)) return invalid("int8_linear: invalid sizes");
     a.tiles = static_cast<int>(tiles);
     a.stage_bytes = round_up(kOperandABytes + a.w_rows * kBlockK, 1024);
