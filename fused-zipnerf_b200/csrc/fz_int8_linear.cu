@@ -21,6 +21,7 @@
 // memory and sets *status.
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_pair.cuh"
 #include "fz_tcgen05.cuh"
 #include "fz_tma.cuh"
 
@@ -91,25 +92,8 @@ __device__ __forceinline__ void mma_int8(const uint32_t d_tmem, const uint64_t a
 // the MMAs issued so far arrive on the barrier when they are done; of a pair, on both CTAs' barriers at this offset
 template <bool kPair>
 __device__ __forceinline__ void commit_to(const uint32_t bar) {
-    if constexpr (kPair) {
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-                     "h"(static_cast<uint16_t>(3))
-                     : "memory");
-    }
+    if constexpr (kPair) commit_pair(bar);
     else commit(bar);
-}
-
-// the address of the pair's first CTA's shared memory at this offset
-__device__ __forceinline__ uint32_t of_first_cta(const uint32_t address) {
-    uint32_t out;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(out) : "r"(address));
-    return out;
-}
-
-// an arrival on a barrier of the cluster; what it orders is tensor memory (fence_before_sync), so it does not wait for
-// this thread's global stores as a release at cluster scope would
-__device__ __forceinline__ void arrive_cluster(const uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // a copy of a pair: into this CTA's shared memory, counted on the first CTA's barrier
@@ -117,10 +101,6 @@ __device__ __forceinline__ void tma_load_2d_pair(const uint32_t dst, const CUten
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                  "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(first_cta_bar)
                  : "memory");
-}
-
-__device__ __forceinline__ void sync_cluster() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // 16 accumulator lanes x 32 columns: of block i of 8 columns, words 4 i, 4 i + 1 are columns 2 (lane % 4), + 1 of row
@@ -330,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (kPair) arrive_cluster(of_first_cta(acc_empty(buffer)));
+                    if constexpr (kPair) arrive_first_cta(acc_empty(buffer));
                     else arrive(acc_empty(buffer));
                 }
             };

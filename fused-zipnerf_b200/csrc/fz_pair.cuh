@@ -1,0 +1,45 @@
+// fz_pair.cuh -- pairs of CTAs (clusters of two whose tcgen05 operations are cta_group::2): commits to both CTAs, arrivals
+// on the first CTA's barriers, tensor-memory stores.
+#pragma once
+
+#include "fz_tcgen05.cuh"
+
+namespace zf::nerf_mlp {
+
+// the pair's MMAs issued so far arrive on both CTAs' barriers at this offset when they are done
+__device__ __forceinline__ void commit_pair(const uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
+}
+
+// the address of the pair's first CTA's shared memory at this offset
+__device__ __forceinline__ uint32_t of_first_cta(const uint32_t address) {
+    uint32_t out;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(out) : "r"(address));
+    return out;
+}
+
+// an arrival on the first CTA's barrier. What it announces lies in the arriving CTA's own tensor memory or shared memory
+// and is read there by the pair's MMAs: fence_before_sync or fence_async_shared before it orders that. A release at cluster
+// scope would wait for this thread's global accesses as well (about 1,000 cycles measured, which bound a pipeline stage).
+__device__ __forceinline__ void arrive_first_cta(const uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(of_first_cta(bar)) : "memory");
+}
+
+__device__ __forceinline__ void sync_cluster() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// 32 consecutive tensor-memory columns of this thread's lane (no wait)
+__device__ __forceinline__ void store_columns(const uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+
+}  // namespace zf::nerf_mlp
