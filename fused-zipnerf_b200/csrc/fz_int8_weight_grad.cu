@@ -8,10 +8,10 @@
 // bf16 twice:
 //   warp 0 (one lane)  brings the stage's codes and gradients by TMA tensor copies (128-byte swizzle, no multicast; rows
 //                      and columns past the tensors arrive as zeros);
-//   warps 2-9          turn the codes into bf16 values codes x scale, the MMAs' second operand; gradients whose rows do
+//   warps 2-17         turn the codes into bf16 values codes x scale, the MMAs' second operand; gradients whose rows do
 //                      not lie on the 16-byte grid they bring too; they sum the bias;
 //   warp 1 (one lane)  of the first CTA issues the MMAs for both;
-//   warps 10-17        add the accumulators to a running sum, every kPeriod stages.
+//   warps 18-25        add the accumulators to a running sum, every kPeriod stages.
 // With power-of-two scales codes x scale is a bf16 number, so both operands are exact and only the sums round. The
 // accumulation in the tensor cores truncates: over one share of 14,000 samples the sums came out 1.5e-5 too small in
 // magnitude (relative; 885 MMA steps). So the accumulator holds 128 MMA steps at a time; the running sum, rounded to
@@ -48,11 +48,12 @@ constexpr int kCodeBytes = kAtomBytes;       // and their codes
 constexpr int kStageBytes = kGradBytes + kCodeBytes;  // what arrives by copies
 constexpr int kStages = 6;                   // enough bytes in flight for the memory's latency
 constexpr int kValueSlots = 4;               // values exist only between the workers and the MMAs
-constexpr int kWorkers = 8;                  // warps that convert
+constexpr int kTeam = 8;                     // warps that convert a stage
+constexpr int kWorkers = 2 * kTeam;          // two teams take alternate stages: a stage's waits are longer than its work
 constexpr int kFirstWorker = 2;
 constexpr int kSummers = 8;                  // warps that read the accumulators
 constexpr int kThreads = 32 * (kFirstWorker + kWorkers + kSummers);
-constexpr int kBiasOffset = 1024;            // behind the barriers: 8 x 128 partial bias sums
+constexpr int kBiasOffset = 1024;            // behind the barriers: 16 x 128 partial bias sums
 constexpr int kRingOffset = kBiasOffset + kWorkers * 128 * 4;
 constexpr int kValueOffset = kRingOffset + kStages * kStageBytes;
 constexpr int kSmemBytes = kValueOffset + kValueSlots * kValueBytes;
@@ -137,7 +138,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(empty_bar(i)), "r"(1));
         }
         for (int i = 0; i < kValueSlots; i++) {
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full_bar(i)), "r"(2 * kWorkers));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(full_bar(i)), "r"(2 * kTeam));
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(sum_bar), "r"(1));
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(read_bar), "r"(2 * kSummers));
@@ -194,22 +195,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
         }
     }
     else if (warp < kFirstWorker + kWorkers) {
-        const int w = warp - kFirstWorker;
+        const int team = (warp - kFirstWorker) / kTeam, w = (warp - kFirstWorker) % kTeam;
         // codes: warp w's rows are 8 w .. 8 w + 7 of a stage; lane l holds row l % 8 and the 16 codes l / 8 of each atom, so
         // that eight lanes of a shared-memory access lie in eight different places of the swizzle
         const int own_row = 8 * w + lane % 8, own_code = 16 * (lane / 8);
-        // the scales of four stages at a time, four stages ahead: lane l holds row 8 w + l % 8 of stage i + l / 8
+        // the scales of four of the team's stages at a time, four of them ahead: lane l holds row 8 w + l % 8 of the
+        // (l / 8)-th
         auto scales_of = [&](const int i) {
-            const int64_t row = row_of(i + lane / 8) + own_row;
-            return i + lane / 8 < stages && row < a.n ? __ldg(a.scales + row) : 0.0f;
+            const int stage = i + 2 * (lane / 8);
+            const int64_t row = row_of(stage) + own_row;
+            return stage < stages && row < a.n ? __ldg(a.scales + row) : 0.0f;
         };
-        // gradients off the grid: warp w's rows w + 8 r, lane l's columns l + 32 j, fetched a stage ahead
-        constexpr int kFetched = kOnGrid ? 1 : kRows / kWorkers * 4;
+        // gradients off the grid: warp w's rows w + 8 r, lane l's columns l + 32 j, fetched one of the team's stages ahead
+        constexpr int kFetched = kOnGrid ? 1 : kRows / kTeam * 4;
         uint16_t next[kFetched];
         auto fetch = [&](const int i) {
             #pragma unroll
             for (int e = 0; e < kFetched; e++) {
-                const int64_t row = row_of(i) + w + kWorkers * (e / 4);
+                const int64_t row = row_of(i) + w + kTeam * (e / 4);
                 const int c = lane + 32 * (e % 4);
                 next[e] = i < stages && row < a.n && c < grad_columns ? __ldg(a.grad + row * a.grad_stride + out0 + c) : static_cast<uint16_t>(0);
             }
@@ -217,15 +220,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
         // bias: on the grid the 8 columns of 16-byte word lane % 16, else columns lane + 32 j; the sum of a stage's rows
         // first, so that the long sum has few steps
         float sums[8] = {};
-        float scales = 0.0f, next_scales = scales_of(0);
-        if (!kOnGrid) fetch(0);
-        for (int i = 0; i < stages; i++) {
+        float scales = 0.0f, next_scales = scales_of(team);
+        if (!kOnGrid) fetch(team);
+        for (int i = team; i < stages; i += 2) {
             const uint32_t slot = i % kStages, value = i % kValueSlots;
-            if (i % 4 == 0) {
+            const int quarter = i / 2 % 4;
+            if (quarter == 0) {
                 scales = next_scales;
-                next_scales = scales_of(i + 4);
+                next_scales = scales_of(i + 8);
             }
-            const uint32_t scale_bits = __float_as_uint(__shfl_sync(0xFFFFFFFFu, scales, i % 4 * 8 + lane % 8));
+            const uint32_t scale_bits = __float_as_uint(__shfl_sync(0xFFFFFFFFu, scales, quarter * 8 + lane % 8));
             const uint64_t scale = static_cast<uint64_t>(scale_bits) << 32 | scale_bits;
             uint8_t* stage = smem + kRingOffset + slot * kStageBytes;
             // warp-uniform, for the shuffle
@@ -257,11 +261,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             if constexpr (!kOnGrid) {
                 #pragma unroll
                 for (int e = 0; e < kFetched; e++) {
-                    const int own = w + kWorkers * (e / 4), c = lane + 32 * (e % 4);
+                    const int own = w + kTeam * (e / 4), c = lane + 32 * (e % 4);
                     *reinterpret_cast<uint16_t*>(stage + c / kAtom * kAtomBytes + own * 128 + (((c % kAtom / 8) ^ (own & 7)) << 4) + c % 8 * 2) = next[e];
                     stage_sums[e % 4] += __uint_as_float(static_cast<uint32_t>(next[e]) << 16);
                 }
-                fetch(i + 1);
+                fetch(i + 2);
             }
             else if (bias && lane % 16 < 8 * grad_atoms) {
                 #pragma unroll
@@ -283,7 +287,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             if (lane == 0) arrive_first_cta(full_bar(value));
         }
         if (bias) {
-            float* partial = reinterpret_cast<float*>(smem + kBiasOffset) + w * 128;
+            float* partial = reinterpret_cast<float*>(smem + kBiasOffset) + (warp - kFirstWorker) * 128;
             if (kOnGrid) {
                 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -298,7 +302,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
         }
     }
     else {
-        // the accumulator's rows 32 quadrant .. + 31, every second 32 columns: added to the running sum, the last time on their way to the workspace,
+        // the accumulator's rows 32 quadrant .. + 31, every second 16 columns: added to the running sum, the last time on their way to the workspace,
         // 4 columns of a row per 16-byte word, neighbouring rows next to one another
         const int quadrant = warp % 4, group = (warp - kFirstWorker - kWorkers) / 4, periods = (stages + kPeriod - 1) / kPeriod;
         const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quadrant) << 16);
@@ -308,19 +312,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             // warp-uniform: the tensor-memory accesses are collective
             if (!__all_sync(0xFFFFFFFFu, wait_phase(sum_bar, p & 1u, abort))) break;
             fence_after_sync();
-            for (int c = 32 * group; c < a.tile_in; c += 64) {
-                uint32_t r[32], sum[32];
-                issue_load<32>(lanes + c, r);
-                if (p > 0) issue_load<32>(lanes + kSumColumn + c, sum);
+            for (int c = 16 * group; c < a.tile_in; c += 32) {
+                uint32_t r[16], sum[16];
+                issue_load<16>(lanes + c, r);
+                if (p > 0) issue_load<16>(lanes + kSumColumn + c, sum);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (p > 0) {
                     #pragma unroll
-                    for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(sum[e]));
+                    for (int e = 0; e < 16; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) + __uint_as_float(sum[e]));
                 }
                 if (p + 1 < periods) store_columns(lanes + kSumColumn + c, r);
                 else if (32 * quadrant < grad_columns) {
                     #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
+                    for (int e = 0; e < 16; e += 4) {
                         to[static_cast<int64_t>((c + e) / 4) * kTileOut] =
                             make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
                     }
