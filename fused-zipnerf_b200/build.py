@@ -111,7 +111,7 @@ def build_torch_extension(force: bool = False) -> Path:
     torch_lib = Path(torch.__file__).resolve().parent / 'lib'
     cmd = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', f'-D_GLIBCXX_USE_CXX11_ABI={abi}', '-DTORCH_EXTENSION_NAME=_C',
            '-DTORCH_API_INCLUDE_EXTENSION_H', f'-I{INCLUDE}', f'-I{python_include}', *[f'-I{p}' for p in includes],
-           str(source), '-o', str(target), f'-L{PACKAGE}', '-lzf_featurize', f'-L{torch_lib}', '-lc10', '-lc10_cuda', '-ltorch',
+           str(source), '-o', str(target), f'-L{PACKAGE}', '-lzf_featurize', f'-L{torch_lib}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cuda',
            '-ltorch_cpu', '-ltorch_python', "-Wl,-rpath,$ORIGIN", f'-Wl,-rpath,{torch_lib}']
     _run(cmd)
     return target

@@ -21,6 +21,7 @@
 // memory and sets *status.
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_launch.h"
 #include "fz_pair.cuh"
 #include "fz_tcgen05.cuh"
 #include "fz_tma.cuh"
@@ -567,7 +568,7 @@ int round_up(const int v, const int to) { return (v + to - 1) / to * to; }
 template <typename Out, bool kRelu, bool kPair>
 cudaError_t launch_kernel(const Args& a, const int n_sms, cudaStream_t stream) {
     const auto kernel = fz_int8_linear_kernel<Out, kRelu, kPair>;
-    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+    const cudaError_t error = zf::allow_shared_memory<fz_int8_linear_kernel<Out, kRelu, kPair>>(kMaxSmem);
     if (error != cudaSuccess) return error;
     constexpr int kCtas = kPair ? 2 : 1;
     cudaLaunchConfig_t config{};
@@ -619,9 +620,8 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
         error = args->output_dtype == ZF_FLOAT32 ? launch_few<float>(f, stream) : launch_few<__nv_bfloat16>(f, stream);
         return error == cudaSuccess ? ZF_OK : zf::set_cuda_error(error, "int8_linear");
     }
-    int device = 0, n_sms = 0;
-    error = cudaGetDevice(&device);
-    if (error == cudaSuccess) error = cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
+    int n_sms = 0;
+    error = zf::current_multiprocessors(&n_sms);
     if (error != cudaSuccess) return zf::set_cuda_error(error, "device query");
     Args a{};
     a.scales = args->scales;

@@ -3,8 +3,9 @@
 // move a few bytes per element and do a few operations on each, so device memory bounds them.
 //
 // A row belongs to a team of kTeam threads (8 lanes, a warp, or a block of 256) of which each holds kHeld elements in
-// registers between the row's reductions, so every input is read once and every output written once. Rows longer than
-// the widest team holds are walked three times by a block (fz_long_* kernels).
+// registers between the row's reductions, so every input is read once and every output written once. A team takes
+// kBatch rows at a time and issues all of their loads, of every operand, before it touches the first value: a conversion
+// behind a load waits for it, and with one load at a time per thread the memory's latency bound these kernels. Rows longer than the widest team holds are walked three times by a block (fz_long_* kernels).
 //
 // Compiled without fast math: the quotients are IEEE ones and subnormal inputs are kept, so that the codes are those of
 // the definition.
@@ -42,30 +43,12 @@ __device__ __forceinline__ void store_one(void* row, const int64_t j, const floa
     else static_cast<__nv_bfloat16*>(row)[j] = __float2bfloat16_rn(v);
 }
 
-// eight elements at the 16-byte aligned address of element j
-template <int kType>
-__device__ __forceinline__ void load_eight(const void* row, const int64_t j, float* v) {
-    if constexpr (kType == kF32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + j);
-        const float4 a = p[0], b = p[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    else {
-        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + j);
-        const uint32_t words[4] = {a.x, a.y, a.z, a.w};
-        #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            v[2 * q] = __uint_as_float(words[q] << 16);
-            v[2 * q + 1] = __uint_as_float(words[q] & 0xFFFF0000u);
-        }
-    }
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(const float lo, const float hi) {
     const __nv_bfloat162 pair = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&pair);
 }
 
+// eight elements at the 16-byte aligned address of element j
 template <int kType>
 __device__ __forceinline__ void store_eight(void* row, const int64_t j, const float* v) {
     if constexpr (kType == kF32) {
@@ -79,15 +62,9 @@ __device__ __forceinline__ void store_eight(void* row, const int64_t j, const fl
     }
 }
 
-__device__ __forceinline__ void load_eight_codes(const int8_t* row, const int64_t j, float* v) {
-    const uint2 a = *reinterpret_cast<const uint2*>(row + j);
-    const uint32_t words[2] = {a.x, a.y};
-    #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = static_cast<float>(static_cast<int8_t>(words[e / 4] >> (8 * (e % 4))));
-}
-
-// reductions over the row's team; every thread of the team gets the result. `shared` holds one word per warp and is
-// free for the next reduction after `barrier`-separated use: the three words of a row alternate between three slots.
+// reductions over the row's team; every thread of the team gets the result. A block's reduction leaves one word per warp
+// in `shared[slot]`; two reductions in a row use different slots, so that the barrier of the second lies between the
+// reads of the first and the next writes to its slot.
 template <int kTeam>
 struct Team {
     uint32_t (*shared)[kBlock / 32];
@@ -125,25 +102,38 @@ struct Team {
 __device__ __forceinline__ uint32_t magnitude_bits(const float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // the scale of a row from the largest magnitude's bits (which order like the magnitudes, infinities and NaN above every
-// finite value), and the factor that turns values into codes
+// finite value), and the factor that turns values into codes: the scale's reciprocal, exact for powers of two, else
+// within an ulp
 __device__ __forceinline__ float row_scale(const uint32_t largest, const bool power_of_two, float& to_codes) {
     to_codes = 0.0f;
     if (largest == 0) return 0.0f;
     if (largest >= kInfinityBits) return __uint_as_float(0x7FFFFFFFu);
-    float scale = fmaxf(__fdiv_rn(__uint_as_float(largest), kLargestCode), kSmallestScale);
     if (power_of_two) {
-        // the next power of two unless it is one: the quotient is at most 2^121, so the exponent has room
-        const uint32_t bits = __float_as_uint(scale);
-        scale = __uint_as_float((bits + 0x007FFFFFu) & 0xFF800000u);
+        // largest / 127 = m 2^e / 127 with 127 = 1.984375 x 2^6: at most 2^(e - 6) exactly when m is at most 1.984375
+        const int exponent = max(static_cast<int>((largest + 0x00020000u - 1u) >> 23) - 6, 1);
+        to_codes = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
+        return __uint_as_float(static_cast<uint32_t>(exponent) << 23);
     }
-    to_codes = __frcp_rn(scale);
+    const float scale = fmaxf(__fdiv_rn(__uint_as_float(largest), kLargestCode), kSmallestScale);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(to_codes) : "f"(scale));
     return scale;
 }
 
-// x / scale to the nearest integer, ties to even. The product with the reciprocal is within 2 ulp of the quotient: at
-// most 127 (1 + 2^-22), so it cannot round to 128; the clamp keeps that true by construction.
-__device__ __forceinline__ int to_code(const float v, const float to_codes) {
-    return max(-127, min(127, __float2int_rn(v * to_codes)));
+// x / scale to the nearest integer, ties to even, in the low byte: the sum with 1.5 x 2^23 leaves the integer in the low
+// bits of the significand, and the product is not rounded before. The product with the reciprocal is within 2 ulp of the
+// quotient: at most 127 (1 + 2^-21), so it cannot round to 128.
+__device__ __forceinline__ uint32_t to_code(const float v, const float to_codes) { return __float_as_uint(fmaf(v, to_codes, 12582912.0f)); }
+
+// the low bytes of four words
+__device__ __forceinline__ uint32_t pack_codes(const uint32_t a, const uint32_t b, const uint32_t c, const uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040u), __byte_perm(c, d, 0x0040u), 0x5410u);
+}
+
+// the larger magnitude (with some sign), NaN if one is
+__device__ __forceinline__ float larger_magnitude(const float a, const float b) {
+    float out;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(out) : "f"(a), "f"(b));
+    return out;
 }
 
 struct QuantizeArgs {
@@ -153,7 +143,7 @@ struct QuantizeArgs {
     int64_t residual_stride;
     const float* weight;
     int64_t n, d;
-    float eps;
+    float one_over_d, eps;
     bool power_of_two;
     int8_t* codes;
     int64_t codes_stride;
@@ -180,27 +170,104 @@ __device__ __forceinline__ int element(const int t, const int i) {
     else return i * kTeam + t;
 }
 
+// a thread's elements of a row as they lie in memory: fetch only loads, value(i) converts. Elements past d are zero.
 template <int kType, bool kVector, int kTeam, int kHeld>
-__device__ __forceinline__ void load_row(const void* row, const int d, const int t, float (&v)[kHeld]) {
-    if constexpr (kVector) {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i += 8) {
-            const int j = element<true, kTeam>(t, i);
-            if (j + 8 <= d) load_eight<kType>(row, j, v + i);
-            else {
+struct Held {
+    static constexpr int kPerWord = kVector && kType == kBf16 ? 2 : 1;
+    uint32_t words[kHeld / kPerWord];
+
+    __device__ __forceinline__ void fetch(const void* row, const int d, const int t) {
+        if constexpr (kVector) {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i += 8) {
+                const int j = element<true, kTeam>(t, i);
+                constexpr int kLoads = kType == kF32 ? 2 : 1;
+                const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + static_cast<int64_t>(j) * kSize<kType>);
                 #pragma unroll
-                for (int e = 0; e < 8; e++) v[i + e] = j + e < d ? load_one<kType>(row, j + e) : 0.0f;
+                for (int q = 0; q < kLoads; q++) {
+                    const uint4 v = j + 8 <= d ? __ldg(from + q) : make_uint4(0, 0, 0, 0);
+                    uint32_t* to = words + i / kPerWord + 4 * q;
+                    to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                }
+            }
+            if (d % 8 != 0) fetch_tail(row, d, t);
+        }
+        else {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) {
+                const int j = element<false, kTeam>(t, i);
+                words[i] = j < d ? bits(row, j) : 0u;
             }
         }
     }
-    else {
+
+    __device__ __forceinline__ float value(const int i) const {
+        if constexpr (kType == kF32) return __uint_as_float(words[i]);
+        else if constexpr (kVector) return __uint_as_float(i % 2 ? words[i / 2] & 0xFFFF0000u : words[i / 2] << 16);
+        else return __uint_as_float(words[i] << 16);
+    }
+
+private:
+    static __device__ __forceinline__ uint32_t bits(const void* row, const int j) {
+        if constexpr (kType == kF32) return __ldg(static_cast<const uint32_t*>(row) + j);
+        else return __ldg(static_cast<const uint16_t*>(row) + j);
+    }
+    // the last d % 8 elements
+    __device__ __forceinline__ void fetch_tail(const void* row, const int d, const int t) {
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            const int j = element<false, kTeam>(t, i);
-            v[i] = j < d ? load_one<kType>(row, j) : 0.0f;
+        for (int i = 0; i < kHeld; i += 8) {
+            const int j = element<true, kTeam>(t, i);
+            if (j >= d || j + 8 <= d) continue;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const uint32_t v = j + e < d ? bits(row, j + e) : 0u;
+                if constexpr (kType == kF32) words[i + e] = v;
+                else words[(i + e) / 2] |= v << (e % 2 * 16);
+            }
         }
     }
-}
+};
+
+// the same for codes
+template <bool kVector, int kTeam, int kHeld>
+struct HeldCodes {
+    uint32_t words[kVector ? kHeld / 4 : kHeld];
+
+    __device__ __forceinline__ void fetch(const int8_t* row, const int d, const int t) {
+        if constexpr (kVector) {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i += 8) {
+                const int j = element<true, kTeam>(t, i);
+                const uint2 v = j + 8 <= d ? __ldg(reinterpret_cast<const uint2*>(row + j)) : make_uint2(0, 0);
+                words[i / 4] = v.x, words[i / 4 + 1] = v.y;
+            }
+            if (d % 8 != 0) {
+                #pragma unroll
+                for (int i = 0; i < kHeld; i += 8) {
+                    const int j = element<true, kTeam>(t, i);
+                    if (j >= d || j + 8 <= d) continue;
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        if (j + e < d) words[(i + e) / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(row + j + e))) << (8 * (e % 4));
+                    }
+                }
+            }
+        }
+        else {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) {
+                const int j = element<false, kTeam>(t, i);
+                words[i] = j < d ? static_cast<uint8_t>(__ldg(row + j)) : 0u;
+            }
+        }
+    }
+
+    // 2^23 + (code + 128) as a float without a conversion instruction, less 2^23 + 128: exact
+    __device__ __forceinline__ float value(const int i) const {
+        const uint32_t biased = (kVector ? words[i / 4] : words[i]) ^ (kVector ? 0x80808080u : 0x80u);
+        return __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440u + (kVector ? i % 4 : 0))) - 8388736.0f;
+    }
+};
 
 template <int kType, bool kVector, int kTeam, int kHeld>
 __device__ __forceinline__ void store_row(void* row, const int d, const int t, const float (&v)[kHeld]) {
@@ -226,98 +293,96 @@ __device__ __forceinline__ void store_row(void* row, const int d, const int t, c
     }
 }
 
-template <bool kVector, int kTeam, int kHeld>
-__device__ __forceinline__ void load_codes(const int8_t* row, const int d, const int t, float (&v)[kHeld]) {
-    if constexpr (kVector) {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i += 8) {
-            const int j = element<true, kTeam>(t, i);
-            if (j + 8 <= d) load_eight_codes(row, j, v + i);
-            else {
-                #pragma unroll
-                for (int e = 0; e < 8; e++) v[i + e] = j + e < d ? static_cast<float>(row[j + e]) : 0.0f;
-            }
-        }
-    }
-    else {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            const int j = element<false, kTeam>(t, i);
-            v[i] = j < d ? static_cast<float>(row[j]) : 0.0f;
-        }
-    }
-}
+// rows that a team fetches before it works on the first: about 32 elements of each operand per thread
+template <int kHeld, int kOperands>
+constexpr int kBatch = kHeld * kOperands >= 32 ? 1 : 32 / (kHeld * kOperands);
 
 // the rows of x (kNorm: the normalised rows of x + residual) as codes and scales
 template <int kX, int kResidual, bool kNorm, bool kVector, int kTeam, int kHeld>
 __global__ void __launch_bounds__(kBlock) fz_quantize_kernel(const QuantizeArgs a) {
+    constexpr int kRows = kBatch<kHeld, kResidual != kNone ? 2 : 1>;
     __shared__ uint32_t shared[2][kBlock / 32];
     const Team<kTeam> team{shared};
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam) + threadIdx.x / kTeam;
-    if (row >= a.n) return;
-    float v[kHeld];
-    load_row<kX, kVector, kTeam>(row_of<kX>(a.x, row, a.x_stride), d, t, v);
-    bool overflow = false;
-    if constexpr (kNorm) {
-        if constexpr (kResidual != kNone) {
-            float r[kHeld];
-            load_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.residual, row, a.residual_stride), d, t, r);
-            #pragma unroll
-            for (int i = 0; i < kHeld; i++) v[i] += r[i];
-            store_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.sum, row, a.sum_stride), d, t, v);
-        }
-        float squares = 0.0f;
-        #pragma unroll
-        for (int i = 0; i < kHeld; i++) squares = fmaf(v[i], v[i], squares);
-        squares = team.sum(squares, 0);
-        overflow = !(squares <= FLT_MAX);
-        const float rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, static_cast<float>(d)) + a.eps));
-        if (t == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
-        #pragma unroll
-        for (int i = 0; i < kHeld; i++) v[i] *= rstd;
-        if (a.weight != nullptr) {
-            #pragma unroll
-            for (int i = 0; i < kHeld; i++) {
-                const int j = element<kVector, kTeam>(t, i);
-                if (j < d) v[i] *= __ldg(a.weight + j);
-            }
-        }
-    }
-    uint32_t largest = 0;
+    // a team's rows: kBlock / kTeam teams of a block side by side, kRows times
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
+    Held<kX, kVector, kTeam, kHeld> x[kRows];
+    Held<kResidual != kNone ? kResidual : kX, kVector, kTeam, kHeld> r[kRows];
     #pragma unroll
-    for (int i = 0; i < kHeld; i++) largest = max(largest, magnitude_bits(v[i]));
-    largest = team.max(largest, 1);
-    if (overflow) largest = kInfinityBits;
-    float to_codes;
-    const float scale = row_scale(largest, a.power_of_two, to_codes);
-    if (t == 0) a.scales[row] = scale;
-    const bool finite = largest < kInfinityBits;
-    int8_t* codes = a.codes + row * a.codes_stride;
-    if constexpr (kVector) {
+    for (int b = 0; b < kRows; b++) {
+        const int64_t row = min(row_at(b), a.n - 1);  // rows past the last repeat it and write nothing
+        x[b].fetch(row_of<kX>(a.x, row, a.x_stride), d, t);
+        if constexpr (kResidual != kNone) r[b].fetch(row_of<kResidual>(a.residual, row, a.residual_stride), d, t);
+    }
+    #pragma unroll
+    for (int b = 0; b < kRows; b++) {
+        const int64_t row = row_at(b);
+        if (row >= a.n) return;
+        float v[kHeld];
         #pragma unroll
-        for (int i = 0; i < kHeld; i += 8) {
-            const int j = element<true, kTeam>(t, i);
-            uint32_t words[2] = {0, 0};
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (finite) words[e / 4] |= (static_cast<uint32_t>(to_code(v[i + e], to_codes)) & 0xFFu) << (8 * (e % 4));
-            }
-            if (j + 8 <= d) *reinterpret_cast<uint2*>(codes + j) = make_uint2(words[0], words[1]);
-            else {
+        for (int i = 0; i < kHeld; i++) v[i] = x[b].value(i);
+        bool overflow = false;
+        if constexpr (kNorm) {
+            if constexpr (kResidual != kNone) {
                 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e / 4] >> (8 * (e % 4)));
+                for (int i = 0; i < kHeld; i++) v[i] += r[b].value(i);
+                store_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.sum, row, a.sum_stride), d, t, v);
+            }
+            float squares = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) squares = fmaf(v[i], v[i], squares);
+            squares = team.sum(squares, 0);
+            overflow = !(squares <= FLT_MAX);
+            const float rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares * a.one_over_d + a.eps);
+            if (t == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) v[i] *= rstd;
+            if (a.weight != nullptr) {
+                #pragma unroll
+                for (int i = 0; i < kHeld; i++) {
+                    const int j = element<kVector, kTeam>(t, i);
+                    if (j < d) v[i] *= __ldg(a.weight + j);
                 }
             }
         }
-    }
-    else {
+        float magnitude = 0.0f;
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            const int j = element<false, kTeam>(t, i);
-            if (j < d) codes[j] = static_cast<int8_t>(finite ? to_code(v[i], to_codes) : 0);
+        for (int i = 0; i < kHeld; i++) magnitude = larger_magnitude(magnitude, v[i]);
+        uint32_t largest = team.max(magnitude_bits(magnitude), kNorm ? 1 : b % 2);
+        if (overflow) largest = kInfinityBits;
+        float to_codes;
+        const float scale = row_scale(largest, a.power_of_two, to_codes);
+        if (t == 0) a.scales[row] = scale;
+        // no code is 0x80 or above 127 in magnitude; those of a row that is not finite are zero
+        const uint32_t keep = largest < kInfinityBits ? 0xFFFFFFFFu : 0u;
+        int8_t* codes = a.codes + row * a.codes_stride;
+        if constexpr (kVector) {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i += 8) {
+                const int j = element<true, kTeam>(t, i);
+                uint32_t words[2];
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float* u = &v[i + 4 * h];
+                    words[h] = pack_codes(to_code(u[0], to_codes), to_code(u[1], to_codes), to_code(u[2], to_codes), to_code(u[3], to_codes)) & keep;
+                }
+                if (j + 8 <= d) *reinterpret_cast<uint2*>(codes + j) = make_uint2(words[0], words[1]);
+                else {
+                    #pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e / 4] >> (8 * (e % 4)));
+                    }
+                }
+            }
+        }
+        else {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) {
+                const int j = element<false, kTeam>(t, i);
+                if (j < d) codes[j] = static_cast<int8_t>(to_code(v[i], to_codes) & keep);
+            }
         }
     }
 }
@@ -345,7 +410,7 @@ __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const Quantize
         }
         squares = team.sum(squares, 0);
         overflow = !(squares <= FLT_MAX);
-        rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(squares, static_cast<float>(a.d)) + a.eps));
+        rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares * a.one_over_d + a.eps);
         if (threadIdx.x == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
     }
     auto scaled = [&](const float v, const int64_t j) {
@@ -365,7 +430,7 @@ __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const Quantize
         const float v = value(j);
         // each thread reads an element of the residual for the last time before it writes the same element of the sum
         if constexpr (kResidual != kNone) store_one<kResidual>(row_of<kResidual>(a.sum, row, a.sum_stride), j, v);
-        codes[j] = static_cast<int8_t>(finite ? to_code(scaled(v, j), to_codes) : 0);
+        codes[j] = static_cast<int8_t>(finite ? to_code(scaled(v, j), to_codes) : 0u);
     }
 }
 
@@ -378,30 +443,56 @@ struct RestoreArgs {
     int64_t out_stride;
 };
 
-// codes * scales, eight (kVector) or one element per thread at a time; blocks of 256 threads over (row, chunk) pairs
-template <int kOut, bool kVector>
+// codes * scales. kVector: a team per row as above, eight elements per access. Else the output, contiguous but with rows
+// off the 16-byte grid, is written as one sequence of 16-byte words, whose elements' rows and columns one division per
+// word finds; or (kWord = 1) any other layout, element by element.
+template <int kOut, int kTeam, int kHeld>
 __global__ void __launch_bounds__(kBlock) fz_dequantize_kernel(const RestoreArgs a) {
-    constexpr int kChunk = kVector ? 8 : 1;
-    const int64_t chunks = (a.d + kChunk - 1) / kChunk;
-    const int64_t total = a.n * chunks;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * kBlock) {
-        const int64_t row = i / chunks, j = (i - row * chunks) * kChunk;
-        const float scale = __ldg(a.scales + row);
-        const int8_t* codes = a.codes + row * a.codes_stride;
-        void* out = row_of<kOut>(a.out, row, a.out_stride);
-        if constexpr (kVector) {
-            if (j + 8 <= a.d) {
-                float v[8];
-                load_eight_codes(codes, j, v);
-                #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] *= scale;
-                store_eight<kOut>(out, j, v);
-            }
+    constexpr int kRows = kBatch<kHeld, 1>;
+    const int t = threadIdx.x % kTeam;
+    const int d = static_cast<int>(a.d);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
+    HeldCodes<true, kTeam, kHeld> codes[kRows];
+    float scales[kRows];
+    #pragma unroll
+    for (int b = 0; b < kRows; b++) {
+        const int64_t row = min(row_at(b), a.n - 1);
+        codes[b].fetch(a.codes + row * a.codes_stride, d, t);
+        scales[b] = __ldg(a.scales + row);
+    }
+    #pragma unroll
+    for (int b = 0; b < kRows; b++) {
+        if (row_at(b) >= a.n) return;
+        float v[kHeld];
+        #pragma unroll
+        for (int i = 0; i < kHeld; i++) v[i] = codes[b].value(i) * scales[b];
+        store_row<kOut, true, kTeam>(row_of<kOut>(a.out, row_at(b), a.out_stride), d, t, v);
+    }
+}
+
+template <int kOut, int kWord>
+__global__ void __launch_bounds__(kBlock) fz_dequantize_flat_kernel(const RestoreArgs a) {
+    const int64_t total = a.n * a.d;
+    for (int64_t at = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * kWord; at < total; at += static_cast<int64_t>(gridDim.x) * kBlock * kWord) {
+        int64_t row = total <= UINT32_MAX ? static_cast<uint32_t>(at) / static_cast<uint32_t>(a.d) : at / a.d;
+        int64_t j = at - row * a.d;
+        float v[kWord];
+        #pragma unroll
+        for (int e = 0; e < kWord; e++) {
+            v[e] = at + e < total ? static_cast<float>(a.codes[row * a.codes_stride + j]) * __ldg(a.scales + row) : 0.0f;
+            if (++j == a.d) j = 0, row++;
+        }
+        if constexpr (kWord == 8) {
+            if (at + 8 <= total) store_eight<kOut>(a.out, at, v);
             else {
-                for (int64_t e = j; e < a.d; e++) store_one<kOut>(out, e, static_cast<float>(codes[e]) * scale);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (at + e < total) store_one<kOut>(a.out, at + e, v[e]);
+                }
             }
         }
-        else store_one<kOut>(out, j, static_cast<float>(codes[j]) * scale);
+        else store_one<kOut>(row_of<kOut>(a.out, at / a.d, a.out_stride), at % a.d, v[0]);
     }
 }
 
@@ -415,6 +506,7 @@ struct BackwardArgs {
     const void* grad_residual;
     int64_t grad_residual_stride;
     int64_t n, d;
+    float one_over_d;
     void* grad_x;
     int64_t grad_x_stride;
 };
@@ -423,31 +515,46 @@ struct BackwardArgs {
 template <int kGrad, int kResidual, bool kVector, int kTeam, int kHeld>
 __global__ void __launch_bounds__(kBlock) fz_norm_backward_kernel(const BackwardArgs a) {
     constexpr int kOut = kResidual != kNone ? kResidual : kGrad;
-    __shared__ uint32_t shared[1][kBlock / 32];
+    constexpr int kRows = kBatch<kHeld, 2>;
+    __shared__ uint32_t shared[2][kBlock / 32];
     const Team<kTeam> team{shared};
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam) + threadIdx.x / kTeam;
-    if (row >= a.n) return;
-    float g[kHeld], y[kHeld];
-    load_row<kGrad, kVector, kTeam>(row_of<kGrad>(a.grad, row, a.grad_stride), d, t, g);
-    load_codes<kVector, kTeam>(a.codes + row * a.codes_stride, d, t, y);
-    float r[kResidual != kNone ? kHeld : 1];
-    if constexpr (kResidual != kNone) load_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.grad_residual, row, a.grad_residual_stride), d, t, r);
-    const float scale = __ldg(a.scales + row), rstd = __ldg(a.rstd + row);
-    float dot = 0.0f;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
+    Held<kGrad, kVector, kTeam, kHeld> grad[kRows];
+    HeldCodes<kVector, kTeam, kHeld> codes[kRows];
+    Held<kOut, kVector, kTeam, kHeld> r[kRows];
+    float scales[kRows], rstds[kRows];
     #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
-        y[i] *= scale;
-        dot = fmaf(g[i], y[i], dot);
+    for (int b = 0; b < kRows; b++) {
+        const int64_t row = min(row_at(b), a.n - 1);  // rows past the last repeat it and write nothing
+        grad[b].fetch(row_of<kGrad>(a.grad, row, a.grad_stride), d, t);
+        codes[b].fetch(a.codes + row * a.codes_stride, d, t);
+        if constexpr (kResidual != kNone) r[b].fetch(row_of<kResidual>(a.grad_residual, row, a.grad_residual_stride), d, t);
+        scales[b] = __ldg(a.scales + row);
+        rstds[b] = __ldg(a.rstd + row);
     }
-    const float mean = __fdiv_rn(team.sum(dot, 0), static_cast<float>(d));
     #pragma unroll
-    for (int i = 0; i < kHeld; i++) {
-        g[i] = rstd * fmaf(-y[i], mean, g[i]);
-        if constexpr (kResidual != kNone) g[i] += r[i];
+    for (int b = 0; b < kRows; b++) {
+        const int64_t row = row_at(b);
+        if (row >= a.n) return;
+        float g[kHeld], y[kHeld];
+        float dot = 0.0f;
+        #pragma unroll
+        for (int i = 0; i < kHeld; i++) {
+            g[i] = grad[b].value(i);
+            y[i] = codes[b].value(i) * scales[b];
+            dot = fmaf(g[i], y[i], dot);
+        }
+        const float mean = team.sum(dot, b % 2) * a.one_over_d;
+        #pragma unroll
+        for (int i = 0; i < kHeld; i++) {
+            g[i] = rstds[b] * fmaf(-y[i], mean, g[i]);
+            if constexpr (kResidual != kNone) g[i] += r[b].value(i);
+        }
+        store_row<kOut, kVector, kTeam>(row_of<kOut>(a.grad_x, row, a.grad_x_stride), d, t, g);
     }
-    store_row<kOut, kVector, kTeam>(row_of<kOut>(a.grad_x, row, a.grad_x_stride), d, t, g);
 }
 
 template <int kGrad, int kResidual>
@@ -461,7 +568,7 @@ __global__ void __launch_bounds__(kBlock) fz_long_norm_backward_kernel(const Bac
     const float scale = __ldg(a.scales + row), rstd = __ldg(a.rstd + row);
     float dot = 0.0f;
     for (int64_t j = threadIdx.x; j < a.d; j += kBlock) dot = fmaf(load_one<kGrad>(grad, j), static_cast<float>(codes[j]) * scale, dot);
-    const float mean = __fdiv_rn(team.sum(dot, 0), static_cast<float>(a.d));
+    const float mean = team.sum(dot, 0) * a.one_over_d;
     void* out = row_of<kOut>(a.grad_x, row, a.grad_x_stride);
     for (int64_t j = threadIdx.x; j < a.d; j += kBlock) {
         float g = rstd * fmaf(-static_cast<float>(codes[j]) * scale, mean, load_one<kGrad>(grad, j));
@@ -504,7 +611,7 @@ cudaError_t launch_quantize(const QuantizeArgs& a, const bool vector, cudaStream
         a.d,
         [&](const auto team, const auto held) {
             constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
-            constexpr int kRows = kBlock / kTeam;
+            constexpr int kRows = kBlock / kTeam * kBatch<kHeld, kResidual != kNone ? 2 : 1>;
             const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
             if (vector) fz_quantize_kernel<kX, kResidual, kNorm, true, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
             else fz_quantize_kernel<kX, kResidual, kNorm, false, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
@@ -519,12 +626,38 @@ cudaError_t launch_backward(const BackwardArgs& a, const bool vector, cudaStream
         a.d,
         [&](const auto team, const auto held) {
             constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
-            constexpr int kRows = kBlock / kTeam;
+            constexpr int kRows = kBlock / kTeam * kBatch<kHeld, 2>;
             const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
             if (vector) fz_norm_backward_kernel<kGrad, kResidual, true, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
             else fz_norm_backward_kernel<kGrad, kResidual, false, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
         },
         [&] { fz_long_norm_backward_kernel<kGrad, kResidual><<<static_cast<unsigned>(a.n), kBlock, 0, stream>>>(a); });
+    return cudaGetLastError();
+}
+
+template <int kOut>
+cudaError_t launch_restore(const RestoreArgs& a, const bool vector, cudaStream_t stream) {
+    // words of eight elements, or single elements, spread over a few blocks per multiprocessor
+    auto flat = [&](const int word) {
+        const int64_t needed = (a.n * a.d + kBlock * word - 1) / (kBlock * word);
+        return static_cast<unsigned>(needed < 4096 ? needed : 4096);
+    };
+    auto element_wise = [&] { fz_dequantize_flat_kernel<kOut, 1><<<flat(1), kBlock, 0, stream>>>(a); };
+    if (vector) {
+        with_team(
+            a.d,
+            [&](const auto team, const auto held) {
+                constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
+                constexpr int kRows = kBlock / kTeam * kBatch<kHeld, 1>;
+                fz_dequantize_kernel<kOut, kTeam, kHeld><<<static_cast<unsigned>((a.n + kRows - 1) / kRows), kBlock, 0, stream>>>(a);
+            },
+            [&] {
+                if (a.out_stride == a.d) fz_dequantize_flat_kernel<kOut, 8><<<flat(8), kBlock, 0, stream>>>(a);
+                else element_wise();
+            });
+    }
+    else if (a.out_stride == a.d && reinterpret_cast<uintptr_t>(a.out) % 16 == 0) fz_dequantize_flat_kernel<kOut, 8><<<flat(8), kBlock, 0, stream>>>(a);
+    else element_wise();
     return cudaGetLastError();
 }
 
@@ -564,24 +697,9 @@ int zf_dequantize_rows(const zf_dequantize_rows_args* args, cudaStream_t stream)
         return invalid("dequantize_rows: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
     if (!valid_rows(args->out, args->out_dtype, args->out_stride, args->d)) return invalid("dequantize_rows: invalid output");
-    int device = 0, n_sms = 0;
-    cudaError_t error = cudaGetDevice(&device);
-    if (error == cudaSuccess) error = cudaDeviceGetAttribute(&n_sms, cudaDevAttrMultiProcessorCount, device);
-    if (error != cudaSuccess) return zf::set_cuda_error(error, "device query");
     const RestoreArgs a{args->codes, args->codes_stride, args->scales, args->n, args->d, args->out, args->out_stride};
     const bool vector = aligned(args->out, args->out_stride, size_of(args->out_dtype));
-    const int64_t chunks = args->n * (vector ? (args->d + 7) / 8 : args->d);
-    const int64_t needed = (chunks + kBlock - 1) / kBlock, most = static_cast<int64_t>(n_sms) * 32;
-    const unsigned blocks = static_cast<unsigned>(needed < most ? needed : most);
-    if (args->out_dtype == ZF_FLOAT32) {
-        if (vector) fz_dequantize_kernel<kF32, true><<<blocks, kBlock, 0, stream>>>(a);
-        else fz_dequantize_kernel<kF32, false><<<blocks, kBlock, 0, stream>>>(a);
-    }
-    else {
-        if (vector) fz_dequantize_kernel<kBf16, true><<<blocks, kBlock, 0, stream>>>(a);
-        else fz_dequantize_kernel<kBf16, false><<<blocks, kBlock, 0, stream>>>(a);
-    }
-    return finish(cudaGetLastError(), "dequantize_rows");
+    return finish(args->out_dtype == ZF_FLOAT32 ? launch_restore<kF32>(a, vector, stream) : launch_restore<kBf16>(a, vector, stream), "dequantize_rows");
 }
 
 int zf_rms_norm_int8(const zf_rms_norm_int8_args* args, cudaStream_t stream) {
@@ -598,7 +716,7 @@ int zf_rms_norm_int8(const zf_rms_norm_int8_args* args, cudaStream_t stream) {
     if (!valid_codes(args->codes, args->codes_stride, args->d) || args->scales == nullptr) {
         return invalid("rms_norm_int8: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
-    const QuantizeArgs a{args->x, args->x_stride, args->residual, args->residual_stride, args->weight, args->n, args->d, args->eps,
+    const QuantizeArgs a{args->x, args->x_stride, args->residual, args->residual_stride, args->weight, args->n, args->d, 1.0f / static_cast<float>(args->d), args->eps,
                          args->power_of_two != 0, args->codes, args->codes_stride, args->scales, args->sum, args->sum_stride, args->rstd};
     const bool residual = args->residual != nullptr;
     const int size = size_of(args->residual_dtype);
@@ -633,7 +751,7 @@ int zf_rms_norm_int8_backward(const zf_rms_norm_int8_backward_args* args, cudaSt
     const int out_dtype = residual ? args->grad_residual_dtype : args->grad_dtype;
     if (!valid_rows(args->grad_x, out_dtype, args->grad_x_stride, args->d)) return invalid("rms_norm_int8_backward: invalid grad_x");
     const BackwardArgs a{args->grad, args->grad_stride, args->codes, args->codes_stride, args->scales, args->rstd, args->grad_residual,
-                         args->grad_residual_stride, args->n, args->d, args->grad_x, args->grad_x_stride};
+                         args->grad_residual_stride, args->n, args->d, 1.0f / static_cast<float>(args->d), args->grad_x, args->grad_x_stride};
     const bool vector = aligned(args->grad, args->grad_stride, size_of(args->grad_dtype)) && aligned(args->grad_x, args->grad_x_stride, size_of(out_dtype))
                         && (!residual || aligned(args->grad_residual, args->grad_residual_stride, size_of(args->grad_residual_dtype)));
     cudaError_t error;

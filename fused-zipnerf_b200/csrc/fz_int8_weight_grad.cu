@@ -23,6 +23,7 @@
 // Bounded waits, pairs and the status as in fz_int8_linear.cu.
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_launch.h"
 #include "fz_pair.cuh"
 #include "fz_tcgen05.cuh"
 #include "fz_tma.cuh"
@@ -491,7 +492,7 @@ bool encode_codes(CUtensorMap* map, const int8_t* codes, const int64_t in, const
 
 template <bool kOnGrid>
 cudaError_t launch(const Args& a, const unsigned blocks, cudaStream_t stream) {
-    const cudaError_t error = cudaFuncSetAttribute(fz_int8_weight_grad_kernel<kOnGrid>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    const cudaError_t error = zf::allow_shared_memory<fz_int8_weight_grad_kernel<kOnGrid>>(kSmemBytes);
     if (error != cudaSuccess) return error;
     fz_int8_weight_grad_kernel<kOnGrid><<<blocks, kThreads, kSmemBytes, stream>>>(a);
     return cudaGetLastError();

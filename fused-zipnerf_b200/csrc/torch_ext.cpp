@@ -17,6 +17,7 @@
 #include "zf_sampling.h"
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -659,8 +660,13 @@ void check_matrix(const at::Tensor& tensor, const char* name) {
     if (!tensor.is_cuda() || tensor.dim() != 2 || tensor.size(1) == 0) throw std::runtime_error(std::string("ZipNeRF: ") + name + " must be a 2D cuda tensor");
 }
 
-at::Tensor empty_codes(const int64_t n, const int64_t d, const at::Tensor& like) {
-    return at::empty({n, (d + 15) / 16 * 16}, like.options().dtype(at::kChar)).narrow(1, 0, d);
+// outputs straight from the allocator: these calls are short, and the dispatcher's part of an allocation would be a
+// noticeable share of them
+at::Tensor empty_rows(const at::IntArrayRef sizes, const at::ScalarType type, const at::Device& device) {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));
+}
+at::Tensor empty_codes(const int64_t n, const int64_t d, const at::Device& device) {
+    return at::Tensor(at::detail::empty_strided_cuda({n, d}, {(d + 15) / 16 * 16, 1}, at::kChar, device));
 }
 
 int8_t* code_ptr(const at::Tensor& codes) { return static_cast<int8_t*>(codes.data_ptr()); }
@@ -689,7 +695,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_rows(const at::Tensor& x, const bool
     a.d = d;
     a.power_of_two = power_of_two ? 1 : 0;
     const c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor codes = empty_codes(n, d, x), scales = at::empty({n}, x.options().dtype(at::kFloat));
+    at::Tensor codes = empty_codes(n, d, x.device()), scales = empty_rows({n}, at::kFloat, x.device());
     a.codes = code_ptr(codes);
     a.codes_stride = (d + 15) / 16 * 16;
     a.scales = scales.data_ptr<float>();
@@ -704,7 +710,7 @@ at::Tensor dequantize_rows(const at::Tensor& codes, const at::Tensor& scales, co
     a.codes_stride = code_stride(codes, "codes", n, d, codes.device());
     check_vector(scales, "scales", n, codes.device());
     const c10::cuda::CUDAGuard guard(codes.device());
-    at::Tensor out = at::empty({n, d}, codes.options().dtype(output_type(dtype)));
+    at::Tensor out = empty_rows({n, d}, output_type(dtype), codes.device());
     a.codes = code_ptr(codes);
     a.scales = scales.data_ptr<float>();
     a.n = n;
@@ -731,7 +737,7 @@ std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>, at::Tensor> rms_no
         a.residual = residual->data_ptr();
         a.residual_dtype = row_type(*residual, "residual");
         a.residual_stride = row_stride(*residual, "residual", n, d, x.device());
-        sum = at::empty({n, d}, residual->options());
+        sum = empty_rows({n, d}, residual->scalar_type(), x.device());
         a.sum = sum->data_ptr();
         a.sum_stride = d;
     }
@@ -743,7 +749,7 @@ std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>, at::Tensor> rms_no
     a.d = d;
     a.eps = static_cast<float>(eps);
     a.power_of_two = power_of_two ? 1 : 0;
-    at::Tensor codes = empty_codes(n, d, x), scales = at::empty({n}, x.options().dtype(at::kFloat)), rstd = at::empty({n}, scales.options());
+    at::Tensor codes = empty_codes(n, d, x.device()), scales = empty_rows({n}, at::kFloat, x.device()), rstd = empty_rows({n}, at::kFloat, x.device());
     a.codes = code_ptr(codes);
     a.codes_stride = (d + 15) / 16 * 16;
     a.scales = scales.data_ptr<float>();
@@ -772,7 +778,7 @@ at::Tensor rms_norm_int8_backward(const at::Tensor& grad, const at::Tensor& code
         a.grad_residual_stride = row_stride(*grad_residual, "grad_residual", n, d, grad.device());
     }
     const c10::cuda::CUDAGuard guard(grad.device());
-    at::Tensor grad_x = at::empty({n, d}, grad_residual.has_value() ? grad_residual->options() : grad.options());
+    at::Tensor grad_x = empty_rows({n, d}, grad_residual.has_value() ? grad_residual->scalar_type() : grad.scalar_type(), grad.device());
     a.n = n;
     a.d = d;
     a.grad_x = grad_x.data_ptr();
@@ -797,7 +803,7 @@ at::Tensor int8_linear(const at::Tensor& codes, const at::Tensor& scales, const 
         a.bias = bias->data_ptr<float>();
     }
     const c10::cuda::CUDAGuard guard(device);
-    at::Tensor output = at::empty({n, out}, codes.options().dtype(output_type(dtype)));
+    at::Tensor output = empty_rows({n, out}, output_type(dtype), device);
     a.codes = code_ptr(codes);
     a.scales = scales.data_ptr<float>();
     a.weight_codes = code_ptr(weight_codes);
@@ -842,7 +848,7 @@ void int8_weight_grad(const at::Tensor& grad, const at::Tensor& codes, const at:
     a.out = out;
     a.grad_weight = grad_weight.data_ptr<float>();
     a.workspace_bytes = zf_int8_weight_grad_workspace_size(n, in, out);
-    const at::Tensor workspace = at::empty({a.workspace_bytes}, grad.options().dtype(at::kByte));
+    const at::Tensor workspace = empty_rows({a.workspace_bytes}, at::kByte, device);
     a.workspace = workspace.data_ptr();
     a.status = int8_status(device).data_ptr<int>();
     check_status(zf_int8_weight_grad(&a, current_stream()));
