@@ -14,11 +14,13 @@
 //   warps 18-25        add the accumulators to a running sum, every kPeriod stages.
 // With power-of-two scales codes x scale is a bf16 number, so both operands are exact and only the sums round. The
 // accumulation in the tensor cores truncates: over one share of 14,000 samples the sums came out 1.5e-5 too small in
-// magnitude (relative; 885 MMA steps). So the accumulator holds 128 MMA steps at a time; the running sum, rounded to
-// nearest, lies beside it in tensor memory (256 + 256 columns), where it needs neither registers nor shared memory.
+// magnitude (relative; 885 MMA steps). So the accumulator holds 48 MMA steps at a time (an error below 1e-6, what a plain
+// fp32 product has; every 128 steps: 2.0e-6, and 4 % faster); the running sum, rounded to nearest, lies beside it in tensor
+// memory (256 + 256 columns), where it needs neither registers nor shared memory.
 //
 // Each CTA leaves its sums in the workspace, in the order of its tensor-memory reads; the join kernel adds the shares of a
-// tile in their order, so that results do not depend on timing.
+// tile in their order, so that results do not depend on timing. It is launched while the first kernel runs and waits for
+// it.
 //
 // Bounded waits, pairs and the status as in fz_int8_linear.cu.
 #include "zf_int8.h"
@@ -38,7 +40,7 @@ namespace zf::int8_weight_grad {
 using namespace zf::nerf_mlp;  // the tcgen05 building blocks
 
 constexpr int kRows = 64;                    // samples of a stage
-constexpr int kPeriod = 32;                  // stages between two additions to the running sum: 128 MMA steps
+constexpr int kPeriod = 12;                  // stages between two additions to the running sum: 48 MMA steps
 constexpr int kAtom = 64;                    // columns of a 128-byte-swizzled atom
 constexpr int kAtomBytes = kRows * 128;
 constexpr int kTileOut = 256;                // outputs of a tile: 128 per CTA
@@ -149,6 +151,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
     }
     fence_before_sync();
     __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join's blocks may be scheduled; they wait for this grid's end
     sync_cluster();  // the other CTA's barriers are ready for remote arrivals
     fence_after_sync();
     const uint32_t tmem = *tmem_slot;
@@ -177,15 +180,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
     else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             const uint32_t idesc = instr_descriptor(kTileOut, a.tile_in, true, true);
+            bool ready = false;
             for (int i = 0; i < stages; i++) {
                 const uint32_t slot = i % kStages, value = i % kValueSlots, parity = (i / kValueSlots) & 1u;
                 // a new period overwrites the accumulator
                 if (i > 0 && i % kPeriod == 0 && !wait_phase(read_bar, (i / kPeriod - 1) & 1u, abort)) break;
-                if (!wait_phase(full_bar(value), parity, abort)) break;
-                if (!wait_phase(landed_bar(slot), (i / kStages) & 1u, abort)) break;  // passed already: the workers waited for it
+                if (!ready && !wait_phase(full_bar(value), parity, abort)) break;
                 fence_after_sync();
                 const uint32_t grad = ring + slot * kStageBytes, values = bar0 + kValueOffset + value * kValueBytes;
+                #pragma unroll
                 for (int k = 0; k < kRows / kMmaK; k++) {
+                    // the next stage is asked for while this one's MMAs run
+                    if (k + 1 == kRows / kMmaK) ready = i + 1 < stages && test_phase(full_bar((i + 1) % kValueSlots), ((i + 1) / kValueSlots) & 1u);
                     // 16 samples: two 8-row groups further
                     mma_pair(tmem, mn_sw128_descriptor(grad + k * 2048, kRows), mn_sw128_descriptor(values + k * 2048, kRows), idesc,
                              (i % kPeriod > 0 || k > 0) ? 1u : 0u);
@@ -207,18 +213,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             const int64_t row = row_of(stage) + own_row;
             return stage < stages && row < a.n ? __ldg(a.scales + row) : 0.0f;
         };
-        // gradients off the grid: warp w's rows w + 8 r, lane l's columns l + 32 j, fetched one of the team's stages ahead
-        constexpr int kFetched = kOnGrid ? 1 : kRows / kTeam * 4;
-        uint16_t next[kFetched];
+        // gradients off the grid: warp w's rows w + 8 r as the aligned 32-bit words that hold them, fetched one of the team's
+        // stages ahead: lane l words l and l + 32, lane 31 word 64 too. A row that begins in the middle of a word is shifted
+        // by 16 bits when it is stored; a warp's rows lie multiples of 8 rows apart, so all of them do or none.
+        constexpr int kFetched = kOnGrid ? 1 : kRows / kTeam;
+        uint32_t next[kFetched][3] = {};
+        const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(a.grad) / 2 + static_cast<uint64_t>(w) * a.grad_stride + out0) & 1);
+        const bool needs[3] = {2 * lane - odd < grad_columns, 2 * (lane + 32) - odd < grad_columns, lane == 31 && 128 - odd < grad_columns};
         auto fetch = [&](const int i) {
+            if (i >= stages) return;
+            const int64_t row0 = row_of(i);
+            const uint16_t* from = a.grad + (row0 + w) * a.grad_stride + out0;
+            if (row0 > 0 && row0 + kRows < a.n) {  // whole words of every row lie in the tensor
+                const uint32_t* words = reinterpret_cast<const uint32_t*>(from - odd) + lane;
+                #pragma unroll
+                for (int r = 0; r < kFetched; r++) {
+                    next[r][0] = needs[0] ? __ldg(words) : 0u;
+                    next[r][1] = needs[1] ? __ldg(words + 32) : 0u;
+                    next[r][2] = needs[2] ? __ldg(words + 33) : 0u;
+                    words += 4 * a.grad_stride;
+                }
+                return;
+            }
             #pragma unroll
-            for (int e = 0; e < kFetched; e++) {
-                const int64_t row = row_of(i) + w + kTeam * (e / 4);
-                const int c = lane + 32 * (e % 4);
-                next[e] = i < stages && row < a.n && c < grad_columns ? __ldg(a.grad + row * a.grad_stride + out0 + c) : static_cast<uint16_t>(0);
+            for (int r = 0; r < kFetched; r++) {
+                const bool live = row0 + w + kTeam * r < a.n;
+                #pragma unroll
+                for (int j = 0; j < 3; j++) {
+                    const int c = 2 * (j == 2 ? 64 : lane + 32 * j) - odd;  // the word's first column
+                    const uint32_t lo = live && needs[j] && c >= 0 ? from[c] : 0u, hi = live && needs[j] && c + 1 < grad_columns ? from[c + 1] : 0u;
+                    next[r][j] = lo | hi << 16;
+                }
+                from += kTeam * a.grad_stride;
             }
         };
-        // bias: on the grid the 8 columns of 16-byte word lane % 16, else columns lane + 32 j; the sum of a stage's rows
+        // bias: on the grid the 8 columns of 16-byte word lane % 16, else columns 2 lane + e % 2 + 64 (e / 2); the sum of a stage's rows
         // first, so that the long sum has few steps
         float sums[8] = {};
         float scales = 0.0f, next_scales = scales_of(team);
@@ -226,10 +255,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
         for (int i = team; i < stages; i += 2) {
             const uint32_t slot = i % kStages, value = i % kValueSlots;
             const int quarter = i / 2 % 4;
-            if (quarter == 0) {
-                scales = next_scales;
-                next_scales = scales_of(i + 8);
-            }
+            if (quarter == 0) scales = next_scales;
             const uint32_t scale_bits = __float_as_uint(__shfl_sync(0xFFFFFFFFu, scales, quarter * 8 + lane % 8));
             const uint64_t scale = static_cast<uint64_t>(scale_bits) << 32 | scale_bits;
             uint8_t* stage = smem + kRingOffset + slot * kStageBytes;
@@ -261,12 +287,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             float stage_sums[8] = {};
             if constexpr (!kOnGrid) {
                 #pragma unroll
-                for (int e = 0; e < kFetched; e++) {
-                    const int own = w + kTeam * (e / 4), c = lane + 32 * (e % 4);
-                    *reinterpret_cast<uint16_t*>(stage + c / kAtom * kAtomBytes + own * 128 + (((c % kAtom / 8) ^ (own & 7)) << 4) + c % 8 * 2) = next[e];
-                    stage_sums[e % 4] += __uint_as_float(static_cast<uint32_t>(next[e]) << 16);
+                for (int r = 0; r < kFetched; r++) {
+                    const int own = w + kTeam * r;  // own & 7 == w
+                    uint32_t pairs[2] = {next[r][0], next[r][1]};
+                    if (odd) {
+                        const uint32_t after0 = __shfl_sync(0xFFFFFFFFu, lane == 0 ? next[r][1] : next[r][0], (lane + 1) % 32);
+                        const uint32_t after1 = __shfl_down_sync(0xFFFFFFFFu, next[r][1], 1);
+                        pairs[0] = __funnelshift_r(next[r][0], after0, 16);
+                        pairs[1] = __funnelshift_r(next[r][1], lane == 31 ? next[r][2] : after1, 16);
+                    }
+                    #pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        *reinterpret_cast<uint32_t*>(stage + j * kAtomBytes + own * 128 + (((lane / 4) ^ w) << 4) + lane % 4 * 4) = pairs[j];
+                        stage_sums[2 * j] += __uint_as_float(pairs[j] << 16);
+                        stage_sums[2 * j + 1] += __uint_as_float(pairs[j] & 0xFFFF0000u);
+                    }
                 }
-                fetch(i + 2);
             }
             else if (bias && lane % 16 < 8 * grad_atoms) {
                 #pragma unroll
@@ -286,6 +322,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             fence_async_shared();
             __syncwarp();
             if (lane == 0) arrive_first_cta(full_bar(value));
+            // behind the fence, which waits for the loads in flight
+            if (quarter == 0) next_scales = scales_of(i + 8);
+            if (!kOnGrid) fetch(i + 2);
         }
         if (bias) {
             float* partial = reinterpret_cast<float*>(smem + kBiasOffset) + (warp - kFirstWorker) * 128;
@@ -298,7 +337,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
             }
             else {
                 #pragma unroll
-                for (int e = 0; e < 4; e++) partial[lane + 32 * e] = sums[e];
+                for (int e = 0; e < 4; e++) partial[2 * lane + e % 2 + e / 2 * 64] = sums[e];
             }
         }
     }
@@ -381,6 +420,7 @@ struct JoinArgs {
 template <bool kSpread>
 __global__ void __launch_bounds__(32 * kJoinWarps) fz_int8_weight_grad_join_kernel(const JoinArgs a) {
     __shared__ float4 parts[kJoinWarps][32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the shares are complete and visible
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (blockIdx.x >= a.word_blocks) {
         const int64_t o = (blockIdx.x - a.word_blocks) * 32 + lane;
@@ -554,10 +594,16 @@ int zf_int8_weight_grad(const zf_int8_weight_grad_args* args, cudaStream_t strea
         const int64_t pieces = p.words() / 32, word_blocks = spread ? pieces : (pieces + kJoinWarps - 1) / kJoinWarps;
         const int64_t bias_blocks = a.bias_partial != nullptr ? (args->out + 31) / 32 : 0;
         const JoinArgs j{a.partial, a.bias_partial, a.in, a.out, a.tile_in, a.tiles_in, a.splits, p.words(), word_blocks, args->grad_weight, args->grad_bias};
-        const unsigned join_blocks = static_cast<unsigned>(word_blocks + bias_blocks);
-        if (spread) fz_int8_weight_grad_join_kernel<true><<<join_blocks, 32 * kJoinWarps, 0, stream>>>(j);
-        else fz_int8_weight_grad_join_kernel<false><<<join_blocks, 32 * kJoinWarps, 0, stream>>>(j);
-        error = cudaGetLastError();
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(static_cast<unsigned>(word_blocks + bias_blocks));
+        config.blockDim = dim3(32 * kJoinWarps);
+        config.stream = stream;
+        cudaLaunchAttribute early{};
+        early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early.val.programmaticStreamSerializationAllowed = 1;
+        config.attrs = &early;
+        config.numAttrs = 1;
+        error = cudaLaunchKernelEx(&config, spread ? fz_int8_weight_grad_join_kernel<true> : fz_int8_weight_grad_join_kernel<false>, j);
     }
     return error == cudaSuccess ? ZF_OK : zf::set_cuda_error(error, "int8_weight_grad");
 }

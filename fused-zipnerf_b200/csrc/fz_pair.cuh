@@ -6,6 +6,16 @@
 
 namespace zf::nerf_mlp {
 
+// whether the phase with the given parity has completed, without waiting
+__device__ __forceinline__ bool test_phase(const uint32_t bar, const uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done != 0;
+}
+
 // the pair's MMAs issued so far arrive on both CTAs' barriers at this offset when they are done
 __device__ __forceinline__ void commit_pair(const uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
