@@ -6,7 +6,8 @@ reference binding (ZipNeRFCudaBackend/ZipNeRFCudaBackend/torch_bindings/bindings
 ``nerf_grid_grad_scale``, ``set_rtc_dirs`` and ``Featurizer``; the sampling functions ``generate_rays``, ``view_rays``,
 ``initialize_rays``, ``sample_uniforms``, ``composite_and_resample``, ``train_final`` and ``composite_final``
 (sampling_api.h:10-90); ``Adam`` (optimizer_api.h:14-40); and the NeRF MLP's ``NerfMlp`` and ``nerf_mlp_parameters``
-(nerf_mlp.h:31-73) with the reference's parameter layout, from ``zipnerf_b200.nerf_mlp`` in the directory above.
+(nerf_mlp.h:31-73) with the reference's parameter layout, from ``zipnerf_b200.nerf_mlp`` in the directory above. The
+8-bit row operators (``quantize_rows`` ... ``int8_status``, include/zf_int8.h) are additions.
 """
 from __future__ import annotations
 
