@@ -14,7 +14,9 @@
 // weight scales and biases of its 16 columns stay in registers over the tiles of a column block. (With a row per lane
 // every column's scale and bias came from shared memory, and those reads were what bound the kernel.) bf16 rows go
 // through a staging tile per warp (stmatrix, 128-byte swizzle) and leave by TMA store when the output lies on the 16-byte
-// grid; fp32 pairs are stored as they are, 32-byte sectors at a time.
+// grid; fp32 pairs are stored as they are, 32-byte sectors at a time. Outputs off the grid whose rows lie back to back
+// (kFlat: an odd width, all outputs in one tile) form one sequence: the four warps of 32 rows stage them together, and one
+// bulk copy writes them, whose start is on the grid again (32 rows). Any other layout is written 32 columns at a time.
 //
 // Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop (the other CTA of
 // a pair runs out on its own); the CTA then waits (bounded) for its own copies and MMAs in flight, frees its tensor
@@ -61,7 +63,8 @@ struct Args {
     int bn, x_rows, w_rows;  // outputs of a tile; operand rows that one CTA loads
     int tiles_n;
     int tiles;
-    int stages, stage_bytes;
+    int stages, stage_bytes, ring_offset;
+    int flat_bytes;          // kFlat: staging of 32 rows
     bool vector;             // output rows on the 16-byte grid
     void* output;
     int64_t output_stride;
@@ -143,7 +146,7 @@ struct Walk {
 };
 
 // kRelu: each output's ReLU, in the conversion for bf16
-template <typename Out, bool kRelu, bool kPair>
+template <typename Out, bool kRelu, bool kPair, bool kFlat>
 __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __grid_constant__ Args a) {
     constexpr int kChunk = 128 / static_cast<int>(sizeof(Out));  // neighbouring columns of one warp
     constexpr int kCtas = kPair ? 2 : 1;
@@ -157,7 +160,9 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     auto acc_full = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + i); };
     auto acc_empty = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + 2 + i); };
     const uint32_t drain_bar = bar0 + 8u * (2 * kMaxStages + 4);
-    const uint32_t ring = smem_address(smem) + kRingOffset;
+    auto staged_bar = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + 5 + i); };    // kFlat, per 32 rows: staged by four warps
+    auto reusable_bar = [&](const uint32_t i) { return bar0 + 8u * (2 * kMaxStages + 9 + i); };  // and read by the copy
+    const uint32_t ring = smem_address(smem) + a.ring_offset;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rank = kPair ? blockIdx.x % 2 : 0;
     const int first_tile = blockIdx.x / kCtas, tile_step = gridDim.x / kCtas;
@@ -184,6 +189,10 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(acc_empty(i)), "r"(kCtas * kEpilogueWarps));
         }
         asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(drain_bar), "r"(1));
+        for (int i = 0; i < 4; i++) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(staged_bar(i)), "r"(kGroups));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(reusable_bar(i)), "r"(1));
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *abort = 0;
     }
@@ -263,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
     }
     else {
         const int group = (warp - kFirstEpilogueWarp) / 4, quadrant = warp % 4;
-        uint8_t* staging = smem + kStagingOffset + (warp - kFirstEpilogueWarp) * kStagingBytes;
+        uint8_t* staging = smem + kStagingOffset + (kFlat ? quadrant * a.flat_bytes : (warp - kFirstEpilogueWarp) * kStagingBytes);
+        uint32_t flat_count = 0;
         const int pair_column = 2 * (lane % 4), lane_row = lane / 4;  // of every 8 columns; of every 8 rows
         // weight scales and biases of this lane's columns: of block b of 8 columns, the chunk's for bf16 (8 blocks), the
         // two chunks' for fp32 (4 blocks each)
@@ -317,7 +327,15 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
             };
             const bool any = group * kChunk < columns && rows > 0;
             if (!any) release();
-            if (sizeof(Out) == 2 && any) {
+            if (kFlat && rows > 0 && flat_count > 0) {
+                // the last sequence's copy has read the staging
+                if (group == kGroups - 1 && lane == 0) {
+                    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    arrive(reusable_bar(quadrant));
+                }
+                if (!__all_sync(0xFFFFFFFFu, wait_phase(reusable_bar(quadrant), (flat_count - 1) & 1u, abort))) break;
+            }
+            if (!kFlat && sizeof(Out) == 2 && any) {
                 // the staging tile's last store has been read
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
@@ -342,7 +360,20 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                             const float2 w = column_scale[i * (kChunk / 8) + b], bias = column_bias[i * (kChunk / 8) + b];
                             const float x = fmaf(static_cast<float>(static_cast<int>(words[b][e])) * s, w.x, bias.x);
                             const float y = fmaf(static_cast<float>(static_cast<int>(words[b][e + 1])) * s, w.y, bias.y);
-                            if constexpr (sizeof(Out) == 2) words[b][e / 2] = kRelu ? pack_bf16x2_relu(x, y) : pack_bf16x2(x, y);
+                            if constexpr (kFlat) {
+                                const int r = 16 * half + 4 * e + lane_row, at = c + 8 * b + pair_column;
+                                Out* to = reinterpret_cast<Out*>(staging) + r * a.out + at;
+                                if constexpr (sizeof(Out) == 4) {
+                                    if (at < columns) to[0] = kRelu ? relu(x) : x;
+                                    if (at + 1 < columns) to[1] = kRelu ? relu(y) : y;
+                                }
+                                else {
+                                    const uint32_t pair = kRelu ? pack_bf16x2_relu(x, y) : pack_bf16x2(x, y);
+                                    if (at < columns) to[0] = __ushort_as_bfloat16(static_cast<uint16_t>(pair));
+                                    if (at + 1 < columns) to[1] = __ushort_as_bfloat16(static_cast<uint16_t>(pair >> 16));
+                                }
+                            }
+                            else if constexpr (sizeof(Out) == 2) words[b][e / 2] = kRelu ? pack_bf16x2_relu(x, y) : pack_bf16x2(x, y);
                             else {
                                 const float u = kRelu ? relu(x) : x, v = kRelu ? relu(y) : y;
                                 const int r = 16 * half + 4 * e + lane_row, at = 8 * b + pair_column;
@@ -357,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                             }
                         }
                     }
-                    if (sizeof(Out) == 4 && half == 1 && !(a.vector && c + kChunk <= columns)) {
+                    if (!kFlat && sizeof(Out) == 4 && half == 1 && !(a.vector && c + kChunk <= columns)) {
                         // rows off the 16-byte grid, or their last columns: 32 neighbouring columns of a row per store
                         __syncwarp();
                         const int first = a.vector ? (columns - c) & ~1 : 0;  // whole pairs are stored already
@@ -374,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                         }
                         __syncwarp();
                     }
-                    if constexpr (sizeof(Out) == 2) {
+                    if constexpr (!kFlat && sizeof(Out) == 2) {
                         // 8 x 8 matrices (block b, rows 0-7), (b, rows 8-15), (b + 1, ...): lane l holds the address of row
                         // l % 8 of matrix l / 8; 16-byte piece p of row r lies at place p ^ (r & 7) of its 128 bytes
                         const int r = 16 * half + lane % 16;
@@ -386,7 +417,25 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     }
                 }
             }
-            if (sizeof(Out) == 2 && any) {
+            if (kFlat && rows > 0) {
+                fence_async_shared();
+                __syncwarp();
+                if (lane == 0) arrive(staged_bar(quadrant));
+                if (group == kGroups - 1) {
+                    if (!__all_sync(0xFFFFFFFFu, wait_phase(staged_bar(quadrant), flat_count & 1u, abort))) break;
+                    if (lane == 0) {
+                        const uint32_t bytes = static_cast<uint32_t>(rows * a.out) * sizeof(Out), whole = bytes & ~15u;
+                        uint8_t* to = static_cast<uint8_t*>(a.output) + static_cast<int64_t>(row0) * a.out * sizeof(Out);
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_address(staging)), "r"(whole) : "memory");
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        // the last rows' last elements
+                        for (uint32_t e = whole; e < bytes; e += sizeof(Out)) *reinterpret_cast<Out*>(to + e) = *reinterpret_cast<const Out*>(staging + e);
+                    }
+                    __syncwarp();
+                }
+                flat_count++;
+            }
+            if (!kFlat && sizeof(Out) == 2 && any) {
                 const int c = group * kChunk;
                 if (a.vector) {
                     fence_async_shared();
@@ -423,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                 }
             }
         }
-        if (sizeof(Out) == 2 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if ((kFlat || sizeof(Out) == 2) && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     // teardown: every role has left its loop; the MMAs already issued finish before the tensor memory is freed
@@ -565,16 +614,16 @@ bool encode_output(CUtensorMap* map, void* output, const int64_t out, const int6
 
 int round_up(const int v, const int to) { return (v + to - 1) / to * to; }
 
-template <typename Out, bool kRelu, bool kPair>
+template <typename Out, bool kRelu, bool kPair, bool kFlat>
 cudaError_t launch_kernel(const Args& a, const int n_sms, cudaStream_t stream) {
-    const auto kernel = fz_int8_linear_kernel<Out, kRelu, kPair>;
-    const cudaError_t error = zf::allow_shared_memory<fz_int8_linear_kernel<Out, kRelu, kPair>>(kMaxSmem);
+    const auto kernel = fz_int8_linear_kernel<Out, kRelu, kPair, kFlat>;
+    const cudaError_t error = zf::allow_shared_memory<fz_int8_linear_kernel<Out, kRelu, kPair, kFlat>>(kMaxSmem);
     if (error != cudaSuccess) return error;
     constexpr int kCtas = kPair ? 2 : 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(kCtas * static_cast<unsigned>(std::min(a.tiles, n_sms / kCtas)));
     config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = kRingOffset + a.stages * a.stage_bytes;
+    config.dynamicSmemBytes = a.ring_offset + a.stages * a.stage_bytes;
     config.stream = stream;
     cudaLaunchAttribute cluster{};
     cluster.id = cudaLaunchAttributeClusterDimension;
@@ -587,7 +636,8 @@ cudaError_t launch_kernel(const Args& a, const int n_sms, cudaStream_t stream) {
 
 template <typename Out, bool kRelu>
 cudaError_t launch(const Args& a, const bool pair, const int n_sms, cudaStream_t stream) {
-    return pair ? launch_kernel<Out, kRelu, true>(a, n_sms, stream) : launch_kernel<Out, kRelu, false>(a, n_sms, stream);
+    if (a.flat_bytes > 0) return pair ? launch_kernel<Out, kRelu, true, true>(a, n_sms, stream) : launch_kernel<Out, kRelu, false, true>(a, n_sms, stream);
+    return pair ? launch_kernel<Out, kRelu, true, false>(a, n_sms, stream) : launch_kernel<Out, kRelu, false, false>(a, n_sms, stream);
 }
 
 int invalid(const char* message) { return zf::set_error(ZF_ERROR_INVALID_ARGUMENT, message); }
@@ -646,8 +696,11 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
     if (tiles > (1 << 30)) return invalid("int8_linear: invalid sizes");
     a.tiles = static_cast<int>(tiles);
     a.stage_bytes = round_up(kOperandABytes + a.w_rows * kBlockK, 1024);
-    a.stages = std::min(kMaxStages, (kMaxSmem - kRingOffset) / a.stage_bytes);
-    a.vector = reinterpret_cast<uintptr_t>(args->output) % 16 == 0 && args->output_stride * size % 16 == 0;
+    const bool aligned = reinterpret_cast<uintptr_t>(args->output) % 16 == 0;
+    a.vector = aligned && args->output_stride * size % 16 == 0;
+    a.flat_bytes = !a.vector && aligned && args->output_stride == args->out && a.tiles_n == 1 ? round_up(32 * a.out * size, 1024) : 0;
+    a.ring_offset = a.flat_bytes > 0 ? kStagingOffset + 4 * a.flat_bytes : kRingOffset;
+    a.stages = std::min(kMaxStages, (kMaxSmem - a.ring_offset) / a.stage_bytes);
     a.output = args->output;
     a.output_stride = args->output_stride;
     a.status = args->status;
