@@ -180,24 +180,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
     else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             const uint32_t idesc = instr_descriptor(kTileOut, a.tile_in, true, true);
+            // one thread's dependent instructions add up to a stage's time: slots, parities and descriptors are carried along
+            // instead of computed from the stage (16 samples, two 8-row groups of 1024 bytes, are 128 further in a descriptor)
+            const uint64_t first_grad = mn_sw128_descriptor(ring, kRows), first_values = mn_sw128_descriptor(bar0 + kValueOffset, kRows);
+            uint64_t grad = first_grad, values = first_values;
+            uint32_t slot = 0, value = 0, parity = 0, in_period = 0, period = 0;
             bool ready = false;
             for (int i = 0; i < stages; i++) {
-                const uint32_t slot = i % kStages, value = i % kValueSlots, parity = (i / kValueSlots) & 1u;
-                // a new period overwrites the accumulator
-                if (i > 0 && i % kPeriod == 0 && !wait_phase(read_bar, (i / kPeriod - 1) & 1u, abort)) break;
+                if (in_period == kPeriod) {  // a new period overwrites the accumulator
+                    if (!wait_phase(read_bar, period & 1u, abort)) break;
+                    period++;
+                    in_period = 0;
+                }
                 if (!ready && !wait_phase(full_bar(value), parity, abort)) break;
                 fence_after_sync();
-                const uint32_t grad = ring + slot * kStageBytes, values = bar0 + kValueOffset + value * kValueBytes;
+                const uint32_t next_value = value + 1 == kValueSlots ? 0 : value + 1, next_parity = next_value == 0 ? parity ^ 1u : parity;
+                mma_pair(tmem, grad, values, idesc, in_period > 0 ? 1u : 0u);
                 #pragma unroll
-                for (int k = 0; k < kRows / kMmaK; k++) {
+                for (int k = 1; k < kRows / kMmaK; k++) {
                     // the next stage is asked for while this one's MMAs run
-                    if (k + 1 == kRows / kMmaK) ready = i + 1 < stages && test_phase(full_bar((i + 1) % kValueSlots), ((i + 1) / kValueSlots) & 1u);
-                    // 16 samples: two 8-row groups further
-                    mma_pair(tmem, mn_sw128_descriptor(grad + k * 2048, kRows), mn_sw128_descriptor(values + k * 2048, kRows), idesc,
-                             (i % kPeriod > 0 || k > 0) ? 1u : 0u);
+                    if (k + 1 == kRows / kMmaK) ready = i + 1 < stages && test_phase(full_bar(next_value), next_parity);
+                    mma_pair(tmem, grad + 128 * k, values + 128 * k, idesc, 1u);
                 }
                 commit_pair(empty_bar(slot));
-                if (i % kPeriod == kPeriod - 1 || i + 1 == stages) commit_pair(sum_bar);
+                if (++in_period == kPeriod || i + 1 == stages) commit_pair(sum_bar);
+                value = next_value;
+                parity = next_parity;
+                values = value == 0 ? first_values : values + kValueBytes / 16;
+                if (++slot == kStages) slot = 0;
+                grad = slot == 0 ? first_grad : grad + kStageBytes / 16;
             }
         }
     }
