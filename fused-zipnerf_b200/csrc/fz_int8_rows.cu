@@ -15,12 +15,17 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cstdint>
 
 namespace zf::int8_rows {
 
 constexpr int kBlock = 256;
+// threads of a team kernel's block: whole teams
+template <int kTeam>
+constexpr int kTeamBlock = kTeam > kBlock || (kTeam > 32 && kTeam < kBlock) ? kTeam : kBlock;
+constexpr int kMaxWarps = 16;
 constexpr float kLargestCode = 127.0f;
 constexpr float kSmallestScale = 0x1p-126f;
 constexpr uint32_t kInfinityBits = 0x7F800000u;
@@ -62,40 +67,52 @@ __device__ __forceinline__ void store_eight(void* row, const int64_t j, const fl
     }
 }
 
-// reductions over the row's team; every thread of the team gets the result. A block's reduction leaves one word per warp
-// in `shared[slot]`; two reductions in a row use different slots, so that the barrier of the second lies between the
-// reads of the first and the next writes to its slot.
-template <int kTeam>
+// reductions over the team's threads, of kRows rows side by side (independent, so their latencies overlap, and a block has
+// one barrier for all of them); every thread gets the results. A block leaves one word per warp and row in `shared`, which
+// serves one reduction.
+template <int kTeam, int kRows>
 struct Team {
-    uint32_t (*shared)[kBlock / 32];
-
-    __device__ __forceinline__ uint32_t mask() const {
+    static __device__ __forceinline__ uint32_t mask() {
         if constexpr (kTeam >= 32) return 0xFFFFFFFFu;
         else return ((1u << kTeam) - 1u) << (threadIdx.x % 32 / kTeam * kTeam);
     }
 
-    __device__ __forceinline__ float sum(float v, const int slot) const {
+    static __device__ __forceinline__ void sum(float (&v)[kRows], uint32_t (&shared)[kRows][kMaxWarps]) {
         #pragma unroll
-        for (int s = (kTeam < 32 ? kTeam : 32) / 2; s > 0; s /= 2) v += __shfl_xor_sync(mask(), v, s);
-        if constexpr (kTeam > 32) {
-            if (threadIdx.x % 32 == 0) shared[slot][threadIdx.x / 32] = __float_as_uint(v);
-            __syncthreads();
-            v = 0.0f;
+        for (int s = (kTeam < 32 ? kTeam : 32) / 2; s > 0; s /= 2) {
             #pragma unroll
-            for (int w = 0; w < kTeam / 32; w++) v += __uint_as_float(shared[slot][w]);
+            for (int b = 0; b < kRows; b++) v[b] += __shfl_xor_sync(mask(), v[b], s);
         }
-        return v;
+        if constexpr (kTeam > 32) {
+            #pragma unroll
+            for (int b = 0; b < kRows; b++) {
+                if (threadIdx.x % 32 == 0) shared[b][threadIdx.x / 32] = __float_as_uint(v[b]);
+            }
+            __syncthreads();
+            #pragma unroll
+            for (int b = 0; b < kRows; b++) {
+                v[b] = 0.0f;
+                #pragma unroll
+                for (int w = 0; w < kTeam / 32; w++) v[b] += __uint_as_float(shared[b][w]);
+            }
+        }
     }
 
-    __device__ __forceinline__ uint32_t max(uint32_t v, const int slot) const {
-        v = __reduce_max_sync(mask(), v);
+    static __device__ __forceinline__ void max(uint32_t (&v)[kRows], uint32_t (&shared)[kRows][kMaxWarps]) {
+        #pragma unroll
+        for (int b = 0; b < kRows; b++) v[b] = __reduce_max_sync(mask(), v[b]);
         if constexpr (kTeam > 32) {
-            if (threadIdx.x % 32 == 0) shared[slot][threadIdx.x / 32] = v;
+            #pragma unroll
+            for (int b = 0; b < kRows; b++) {
+                if (threadIdx.x % 32 == 0) shared[b][threadIdx.x / 32] = v[b];
+            }
             __syncthreads();
             #pragma unroll
-            for (int w = 0; w < kTeam / 32; w++) v = ::max(v, shared[slot][w]);
+            for (int b = 0; b < kRows; b++) {
+                #pragma unroll
+                for (int w = 0; w < kTeam / 32; w++) v[b] = ::max(v[b], shared[b][w]);
+            }
         }
-        return v;
     }
 };
 
@@ -162,48 +179,57 @@ __device__ __forceinline__ void* row_of(void* base, const int64_t row, const int
     return static_cast<uint8_t*>(base) + row * stride * kSize<kType>;
 }
 
-// element i of thread t of a team: kVector: eight neighbouring elements per 16-byte (bf16) access, else one at a time
-// with neighbouring threads on neighbouring elements
-template <bool kVector, int kTeam>
+// element i of thread t of a team. kVector neighbouring elements go with one access, neighbouring threads on neighbouring
+// accesses: 8 where the rows lie on the 16-byte grid, 2 where they lie on pairs of elements (an even width), else 1.
+template <int kVector, int kTeam>
 __device__ __forceinline__ int element(const int t, const int i) {
-    if constexpr (kVector) return (i / 8) * (8 * kTeam) + 8 * t + i % 8;
-    else return i * kTeam + t;
+    return i / kVector * (kVector * kTeam) + kVector * t + i % kVector;
 }
 
 // a thread's elements of a row as they lie in memory: fetch only loads, value(i) converts. Elements past d are zero.
-template <int kType, bool kVector, int kTeam, int kHeld>
+template <int kType, int kVector, int kTeam, int kHeld>
 struct Held {
-    static constexpr int kPerWord = kVector && kType == kBf16 ? 2 : 1;
+    static constexpr int kPerWord = kVector > 1 && kType == kBf16 ? 2 : 1;
     uint32_t words[kHeld / kPerWord];
 
     __device__ __forceinline__ void fetch(const void* row, const int d, const int t) {
-        if constexpr (kVector) {
-            #pragma unroll
-            for (int i = 0; i < kHeld; i += 8) {
-                const int j = element<true, kTeam>(t, i);
-                constexpr int kLoads = kType == kF32 ? 2 : 1;
-                const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + static_cast<int64_t>(j) * kSize<kType>);
+        #pragma unroll
+        for (int i = 0; i < kHeld; i += kVector) {
+            const int j = element<kVector, kTeam>(t, i);
+            const uint8_t* from = static_cast<const uint8_t*>(row) + static_cast<int64_t>(j) * kSize<kType>;
+            uint32_t* to = words + i / kPerWord;
+            if constexpr (kVector == 8) {
                 #pragma unroll
-                for (int q = 0; q < kLoads; q++) {
-                    const uint4 v = j + 8 <= d ? __ldg(from + q) : make_uint4(0, 0, 0, 0);
-                    uint32_t* to = words + i / kPerWord + 4 * q;
-                    to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+                for (int q = 0; q < 2 / kPerWord; q++) {
+                    const uint4 v = j + 8 <= d ? __ldg(reinterpret_cast<const uint4*>(from) + q) : make_uint4(0, 0, 0, 0);
+                    to[4 * q] = v.x, to[4 * q + 1] = v.y, to[4 * q + 2] = v.z, to[4 * q + 3] = v.w;
                 }
             }
-            if (d % 8 != 0) fetch_tail(row, d, t);
+            else if constexpr (kVector == 2 && kType == kF32) {
+                const uint2 v = j + 2 <= d ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
+                to[0] = v.x, to[1] = v.y;
+            }
+            else if constexpr (kVector == 2) to[0] = j + 2 <= d ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0u;
+            else to[0] = j < d ? bits(row, j) : 0u;
         }
-        else {
+        if (kVector > 1 && d % kVector != 0) {  // the last elements, in the team's thread whose access they do not fill
             #pragma unroll
-            for (int i = 0; i < kHeld; i++) {
-                const int j = element<false, kTeam>(t, i);
-                words[i] = j < d ? bits(row, j) : 0u;
+            for (int i = 0; i < kHeld; i += kVector) {
+                const int j = element<kVector, kTeam>(t, i);
+                if (j >= d || j + kVector <= d) continue;
+                #pragma unroll
+                for (int e = 0; e < kVector; e++) {
+                    const uint32_t v = j + e < d ? bits(row, j + e) : 0u;
+                    if constexpr (kPerWord == 1) words[i + e] = v;
+                    else words[(i + e) / 2] |= v << (e % 2 * 16);
+                }
             }
         }
     }
 
     __device__ __forceinline__ float value(const int i) const {
         if constexpr (kType == kF32) return __uint_as_float(words[i]);
-        else if constexpr (kVector) return __uint_as_float(i % 2 ? words[i / 2] & 0xFFFF0000u : words[i / 2] << 16);
+        else if constexpr (kPerWord == 2) return __uint_as_float(i % 2 ? words[i / 2] & 0xFFFF0000u : words[i / 2] << 16);
         else return __uint_as_float(words[i] << 16);
     }
 
@@ -212,102 +238,86 @@ private:
         if constexpr (kType == kF32) return __ldg(static_cast<const uint32_t*>(row) + j);
         else return __ldg(static_cast<const uint16_t*>(row) + j);
     }
-    // the last d % 8 elements
-    __device__ __forceinline__ void fetch_tail(const void* row, const int d, const int t) {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i += 8) {
-            const int j = element<true, kTeam>(t, i);
-            if (j >= d || j + 8 <= d) continue;
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t v = j + e < d ? bits(row, j + e) : 0u;
-                if constexpr (kType == kF32) words[i + e] = v;
-                else words[(i + e) / 2] |= v << (e % 2 * 16);
-            }
-        }
-    }
 };
 
-// the same for codes
-template <bool kVector, int kTeam, int kHeld>
+// the same for codes: kVector of them in kWords words
+template <int kVector, int kTeam, int kHeld>
 struct HeldCodes {
-    uint32_t words[kVector ? kHeld / 4 : kHeld];
+    static constexpr int kPerWord = kVector == 8 ? 4 : kVector;
+    uint32_t words[kHeld / kPerWord];
 
     __device__ __forceinline__ void fetch(const int8_t* row, const int d, const int t) {
-        if constexpr (kVector) {
-            #pragma unroll
-            for (int i = 0; i < kHeld; i += 8) {
-                const int j = element<true, kTeam>(t, i);
+        #pragma unroll
+        for (int i = 0; i < kHeld; i += kVector) {
+            const int j = element<kVector, kTeam>(t, i);
+            uint32_t* to = words + i / kPerWord;
+            if constexpr (kVector == 8) {
                 const uint2 v = j + 8 <= d ? __ldg(reinterpret_cast<const uint2*>(row + j)) : make_uint2(0, 0);
-                words[i / 4] = v.x, words[i / 4 + 1] = v.y;
+                to[0] = v.x, to[1] = v.y;
             }
-            if (d % 8 != 0) {
-                #pragma unroll
-                for (int i = 0; i < kHeld; i += 8) {
-                    const int j = element<true, kTeam>(t, i);
-                    if (j >= d || j + 8 <= d) continue;
-                    #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if (j + e < d) words[(i + e) / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(row + j + e))) << (8 * (e % 4));
-                    }
-                }
-            }
+            else if constexpr (kVector == 2) to[0] = j + 2 <= d ? __ldg(reinterpret_cast<const uint16_t*>(row + j)) : 0u;
+            else to[0] = j < d ? static_cast<uint8_t>(__ldg(row + j)) : 0u;
         }
-        else {
+        if (kVector > 1 && d % kVector != 0) {
             #pragma unroll
-            for (int i = 0; i < kHeld; i++) {
-                const int j = element<false, kTeam>(t, i);
-                words[i] = j < d ? static_cast<uint8_t>(__ldg(row + j)) : 0u;
+            for (int i = 0; i < kHeld; i += kVector) {
+                const int j = element<kVector, kTeam>(t, i);
+                if (j >= d || j + kVector <= d) continue;
+                #pragma unroll
+                for (int e = 0; e < kVector; e++) {
+                    if (j + e < d) words[(i + e) / kPerWord] |= static_cast<uint32_t>(static_cast<uint8_t>(__ldg(row + j + e))) << (8 * (e % kPerWord));
+                }
             }
         }
     }
 
     // 2^23 + (code + 128) as a float without a conversion instruction, less 2^23 + 128: exact
     __device__ __forceinline__ float value(const int i) const {
-        const uint32_t biased = (kVector ? words[i / 4] : words[i]) ^ (kVector ? 0x80808080u : 0x80u);
-        return __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7440u + (kVector ? i % 4 : 0))) - 8388736.0f;
+        return __uint_as_float(__byte_perm(words[i / kPerWord] ^ 0x80808080u, 0x4B000000u, 0x7440u + i % kPerWord)) - 8388736.0f;
     }
 };
 
-template <int kType, bool kVector, int kTeam, int kHeld>
+template <int kType, int kVector, int kTeam, int kHeld>
 __device__ __forceinline__ void store_row(void* row, const int d, const int t, const float (&v)[kHeld]) {
-    if constexpr (kVector) {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i += 8) {
-            const int j = element<true, kTeam>(t, i);
-            if (j + 8 <= d) store_eight<kType>(row, j, v + i);
-            else {
-                #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if (j + e < d) store_one<kType>(row, j + e, v[i + e]);
-                }
+    #pragma unroll
+    for (int i = 0; i < kHeld; i += kVector) {
+        const int j = element<kVector, kTeam>(t, i);
+        if (j + kVector <= d) {
+            if constexpr (kVector == 8) store_eight<kType>(row, j, v + i);
+            else if constexpr (kVector == 2 && kType == kF32) *reinterpret_cast<float2*>(static_cast<float*>(row) + j) = make_float2(v[i], v[i + 1]);
+            else if constexpr (kVector == 2) *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(row) + j) = pack_bf16(v[i], v[i + 1]);
+            else store_one<kType>(row, j, v[i]);
+        }
+        else {
+            #pragma unroll
+            for (int e = 0; e + 1 < kVector; e++) {
+                if (j + e < d) store_one<kType>(row, j + e, v[i + e]);
             }
         }
     }
-    else {
-        #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            const int j = element<false, kTeam>(t, i);
-            if (j < d) store_one<kType>(row, j, v[i]);
-        }
-    }
 }
+
+// rows that a team reduces side by side: a block all of its batch (one barrier), fewer threads one after the other (a row's
+// stores leave while the next is worked on: 5 to 10 % faster at 256 columns)
+template <int kTeam, int kRows>
+constexpr int kTogether = kTeam > 32 ? kRows : 1;
 
 // rows that a team fetches before it works on the first: about 32 elements of each operand per thread
 template <int kHeld, int kOperands>
 constexpr int kBatch = kHeld * kOperands >= 32 ? 1 : 32 / (kHeld * kOperands);
 
 // the rows of x (kNorm: the normalised rows of x + residual) as codes and scales
-template <int kX, int kResidual, bool kNorm, bool kVector, int kTeam, int kHeld>
-__global__ void __launch_bounds__(kBlock) fz_quantize_kernel(const QuantizeArgs a) {
+template <int kX, int kResidual, bool kNorm, int kVector, int kTeam, int kHeld>
+__global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_quantize_kernel(const QuantizeArgs a) {
     constexpr int kRows = kBatch<kHeld, kResidual != kNone ? 2 : 1>;
-    __shared__ uint32_t shared[2][kBlock / 32];
-    const Team<kTeam> team{shared};
+    __shared__ uint32_t shared[2][kTogether<kTeam, kRows>][kMaxWarps];
+    constexpr int kSide = kTogether<kTeam, kRows>;
+    using Rows = Team<kTeam, kSide>;
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
-    // a team's rows: kBlock / kTeam teams of a block side by side, kRows times
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
-    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
+    // a team's rows: the teams of a block side by side, kRows times
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kTeamBlock<kTeam> / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kTeamBlock<kTeam> / kTeam); };
     Held<kX, kVector, kTeam, kHeld> x[kRows];
     Held<kResidual != kNone ? kResidual : kX, kVector, kTeam, kHeld> r[kRows];
     #pragma unroll
@@ -317,71 +327,81 @@ __global__ void __launch_bounds__(kBlock) fz_quantize_kernel(const QuantizeArgs 
         if constexpr (kResidual != kNone) r[b].fetch(row_of<kResidual>(a.residual, row, a.residual_stride), d, t);
     }
     #pragma unroll
-    for (int b = 0; b < kRows; b++) {
-        const int64_t row = row_at(b);
-        if (row >= a.n) return;
-        float v[kHeld];
+    for (int of = 0; of < kRows; of += kSide) {
+        float v[kSide][kHeld];
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) v[i] = x[b].value(i);
-        bool overflow = false;
-        if constexpr (kNorm) {
+        for (int b = 0; b < kSide; b++) {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) v[b][i] = kResidual != kNone ? x[of + b].value(i) + r[of + b].value(i) : x[of + b].value(i);
             if constexpr (kResidual != kNone) {
-                #pragma unroll
-                for (int i = 0; i < kHeld; i++) v[i] += r[b].value(i);
-                store_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.sum, row, a.sum_stride), d, t, v);
+                if (row_at(of + b) < a.n) store_row<kResidual, kVector, kTeam>(row_of<kResidual>(a.sum, row_at(of + b), a.sum_stride), d, t, v[b]);
             }
-            float squares = 0.0f;
+        }
+        bool overflow[kSide] = {};
+        if constexpr (kNorm) {
+            float squares[kSide] = {};
             #pragma unroll
-            for (int i = 0; i < kHeld; i++) squares = fmaf(v[i], v[i], squares);
-            squares = team.sum(squares, 0);
-            overflow = !(squares <= FLT_MAX);
-            const float rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares * a.one_over_d + a.eps);
-            if (t == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
+            for (int b = 0; b < kSide; b++) {
+                #pragma unroll
+                for (int i = 0; i < kHeld; i++) squares[b] = fmaf(v[b][i], v[b][i], squares[b]);
+            }
+            Rows::sum(squares, shared[0]);
             #pragma unroll
-            for (int i = 0; i < kHeld; i++) v[i] *= rstd;
+            for (int b = 0; b < kSide; b++) {
+                overflow[b] = !(squares[b] <= FLT_MAX);
+                const float rstd = overflow[b] ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares[b] * a.one_over_d + a.eps);
+                if (t == 0 && a.rstd != nullptr && row_at(of + b) < a.n) a.rstd[row_at(of + b)] = rstd;
+                #pragma unroll
+                for (int i = 0; i < kHeld; i++) v[b][i] *= rstd;
+            }
             if (a.weight != nullptr) {
                 #pragma unroll
                 for (int i = 0; i < kHeld; i++) {
                     const int j = element<kVector, kTeam>(t, i);
-                    if (j < d) v[i] *= __ldg(a.weight + j);
+                    const float weight = j < d ? __ldg(a.weight + j) : 0.0f;
+                    #pragma unroll
+                    for (int b = 0; b < kSide; b++) v[b][i] *= weight;
                 }
             }
         }
-        float magnitude = 0.0f;
+        uint32_t largest[kSide];
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) magnitude = larger_magnitude(magnitude, v[i]);
-        uint32_t largest = team.max(magnitude_bits(magnitude), kNorm ? 1 : b % 2);
-        if (overflow) largest = kInfinityBits;
-        float to_codes;
-        const float scale = row_scale(largest, a.power_of_two, to_codes);
-        if (t == 0) a.scales[row] = scale;
-        // no code is 0x80 or above 127 in magnitude; those of a row that is not finite are zero
-        const uint32_t keep = largest < kInfinityBits ? 0xFFFFFFFFu : 0u;
-        int8_t* codes = a.codes + row * a.codes_stride;
-        if constexpr (kVector) {
+        for (int b = 0; b < kSide; b++) {
+            float magnitude = 0.0f;
             #pragma unroll
-            for (int i = 0; i < kHeld; i += 8) {
-                const int j = element<true, kTeam>(t, i);
-                uint32_t words[2];
+            for (int i = 0; i < kHeld; i++) magnitude = larger_magnitude(magnitude, v[b][i]);
+            largest[b] = magnitude_bits(magnitude);
+        }
+        Rows::max(largest, shared[1]);
+        #pragma unroll
+        for (int b = 0; b < kSide; b++) {
+            const int64_t row = row_at(of + b);
+            if (row >= a.n) return;
+            if (overflow[b]) largest[b] = kInfinityBits;
+            float to_codes;
+            const float scale = row_scale(largest[b], a.power_of_two, to_codes);
+            if (t == 0) a.scales[row] = scale;
+            const uint32_t keep = largest[b] < kInfinityBits ? 0xFFFFFFFFu : 0u;  // the codes of a row that is not finite are zero
+            int8_t* codes = a.codes + row * a.codes_stride;
+            #pragma unroll
+            for (int i = 0; i < kHeld; i += kVector) {
+                const int j = element<kVector, kTeam>(t, i);
+                uint32_t words[kVector];
                 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const float* u = &v[i + 4 * h];
-                    words[h] = pack_codes(to_code(u[0], to_codes), to_code(u[1], to_codes), to_code(u[2], to_codes), to_code(u[3], to_codes)) & keep;
+                for (int e = 0; e < kVector; e++) words[e] = to_code(v[b][i + e], to_codes) & keep;
+                if (j + kVector <= d) {
+                    if constexpr (kVector == 8) {
+                        *reinterpret_cast<uint2*>(codes + j) = make_uint2(pack_codes(words[0], words[1], words[2], words[3]), pack_codes(words[4], words[5], words[6], words[7]));
+                    }
+                    else if constexpr (kVector == 2) *reinterpret_cast<uint16_t*>(codes + j) = static_cast<uint16_t>(__byte_perm(words[0], words[1], 0x0040u));
+                    else codes[j] = static_cast<int8_t>(words[0]);
                 }
-                if (j + 8 <= d) *reinterpret_cast<uint2*>(codes + j) = make_uint2(words[0], words[1]);
                 else {
                     #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e / 4] >> (8 * (e % 4)));
+                    for (int e = 0; e + 1 < kVector; e++) {
+                        if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e]);
                     }
                 }
-            }
-        }
-        else {
-            #pragma unroll
-            for (int i = 0; i < kHeld; i++) {
-                const int j = element<false, kTeam>(t, i);
-                if (j < d) codes[j] = static_cast<int8_t>(to_code(v[i], to_codes) & keep);
             }
         }
     }
@@ -390,8 +410,8 @@ __global__ void __launch_bounds__(kBlock) fz_quantize_kernel(const QuantizeArgs 
 // rows longer than a team holds: a block reads the row once per reduction and once more for the codes
 template <int kX, int kResidual, bool kNorm>
 __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const QuantizeArgs a) {
-    __shared__ uint32_t shared[2][kBlock / 32];
-    const Team<kBlock> team{shared};
+    __shared__ uint32_t shared[2][1][kMaxWarps];
+    using Row = Team<kBlock, 1>;
     const int64_t row = blockIdx.x;
     const void* x = row_of<kX>(a.x, row, a.x_stride);
     const void* residual = kResidual != kNone ? row_of<kResidual>(a.residual, row, a.residual_stride) : nullptr;
@@ -403,28 +423,28 @@ __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const Quantize
     float rstd = 1.0f;
     bool overflow = false;
     if constexpr (kNorm) {
-        float squares = 0.0f;
+        float squares[1] = {0.0f};
         for (int64_t j = threadIdx.x; j < a.d; j += kBlock) {
             const float v = value(j);
-            squares = fmaf(v, v, squares);
+            squares[0] = fmaf(v, v, squares[0]);
         }
-        squares = team.sum(squares, 0);
-        overflow = !(squares <= FLT_MAX);
-        rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares * a.one_over_d + a.eps);
+        Row::sum(squares, shared[0]);
+        overflow = !(squares[0] <= FLT_MAX);
+        rstd = overflow ? __uint_as_float(0x7FFFFFFFu) : __frsqrt_rn(squares[0] * a.one_over_d + a.eps);
         if (threadIdx.x == 0 && a.rstd != nullptr) a.rstd[row] = rstd;
     }
     auto scaled = [&](const float v, const int64_t j) {
         if constexpr (!kNorm) return v;
         else return a.weight != nullptr ? v * rstd * __ldg(a.weight + j) : v * rstd;
     };
-    uint32_t largest = 0;
-    for (int64_t j = threadIdx.x; j < a.d; j += kBlock) largest = max(largest, magnitude_bits(scaled(value(j), j)));
-    largest = team.max(largest, 1);
-    if (overflow) largest = kInfinityBits;
+    uint32_t largest[1] = {0};
+    for (int64_t j = threadIdx.x; j < a.d; j += kBlock) largest[0] = max(largest[0], magnitude_bits(scaled(value(j), j)));
+    Row::max(largest, shared[1]);
+    if (overflow) largest[0] = kInfinityBits;
     float to_codes;
-    const float scale = row_scale(largest, a.power_of_two, to_codes);
+    const float scale = row_scale(largest[0], a.power_of_two, to_codes);
     if (threadIdx.x == 0) a.scales[row] = scale;
-    const bool finite = largest < kInfinityBits;
+    const bool finite = largest[0] < kInfinityBits;
     int8_t* codes = a.codes + row * a.codes_stride;
     for (int64_t j = threadIdx.x; j < a.d; j += kBlock) {
         const float v = value(j);
@@ -447,13 +467,13 @@ struct RestoreArgs {
 // off the 16-byte grid, is written as one sequence of 16-byte words, whose elements' rows and columns one division per
 // word finds; or (kWord = 1) any other layout, element by element.
 template <int kOut, int kTeam, int kHeld>
-__global__ void __launch_bounds__(kBlock) fz_dequantize_kernel(const RestoreArgs a) {
+__global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_dequantize_kernel(const RestoreArgs a) {
     constexpr int kRows = kBatch<kHeld, 1>;
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
-    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
-    HeldCodes<true, kTeam, kHeld> codes[kRows];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kTeamBlock<kTeam> / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kTeamBlock<kTeam> / kTeam); };
+    HeldCodes<8, kTeam, kHeld> codes[kRows];
     float scales[kRows];
     #pragma unroll
     for (int b = 0; b < kRows; b++) {
@@ -467,7 +487,7 @@ __global__ void __launch_bounds__(kBlock) fz_dequantize_kernel(const RestoreArgs
         float v[kHeld];
         #pragma unroll
         for (int i = 0; i < kHeld; i++) v[i] = codes[b].value(i) * scales[b];
-        store_row<kOut, true, kTeam>(row_of<kOut>(a.out, row_at(b), a.out_stride), d, t, v);
+        store_row<kOut, 8, kTeam>(row_of<kOut>(a.out, row_at(b), a.out_stride), d, t, v);
     }
 }
 
@@ -478,10 +498,22 @@ __global__ void __launch_bounds__(kBlock) fz_dequantize_flat_kernel(const Restor
         int64_t row = total <= UINT32_MAX ? static_cast<uint32_t>(at) / static_cast<uint32_t>(a.d) : at / a.d;
         int64_t j = at - row * a.d;
         float v[kWord];
-        #pragma unroll
-        for (int e = 0; e < kWord; e++) {
-            v[e] = at + e < total ? static_cast<float>(a.codes[row * a.codes_stride + j]) * __ldg(a.scales + row) : 0.0f;
-            if (++j == a.d) j = 0, row++;
+        if (kWord == 8 && j + 8 <= a.d && row + 1 < a.n) {
+            // eight codes of one row, from the aligned words around them (the last may reach into the next row)
+            const uint32_t* words = reinterpret_cast<const uint32_t*>(a.codes + row * a.codes_stride + (j & ~int64_t{3}));
+            const uint32_t shift = static_cast<uint32_t>(j & 3) * 8;
+            const uint32_t w0 = __ldg(words), w1 = __ldg(words + 1), w2 = shift != 0 ? __ldg(words + 2) : 0u;
+            const uint32_t eight[2] = {__funnelshift_r(w0, w1, shift) ^ 0x80808080u, __funnelshift_r(w1, w2, shift) ^ 0x80808080u};
+            const float scale = __ldg(a.scales + row);
+            #pragma unroll
+            for (int e = 0; e < kWord; e++) v[e] = (__uint_as_float(__byte_perm(eight[e / 4 % 2], 0x4B000000u, 0x7440u + e % 4)) - 8388736.0f) * scale;
+        }
+        else {
+            #pragma unroll
+            for (int e = 0; e < kWord; e++) {
+                v[e] = at + e < total ? static_cast<float>(a.codes[row * a.codes_stride + j]) * __ldg(a.scales + row) : 0.0f;
+                if (++j == a.d) j = 0, row++;
+            }
         }
         if constexpr (kWord == 8) {
             if (at + 8 <= total) store_eight<kOut>(a.out, at, v);
@@ -512,16 +544,16 @@ struct BackwardArgs {
 };
 
 // grad_x = rstd (grad - y mean(grad y)) + grad_residual, y = codes * scale
-template <int kGrad, int kResidual, bool kVector, int kTeam, int kHeld>
-__global__ void __launch_bounds__(kBlock) fz_norm_backward_kernel(const BackwardArgs a) {
+template <int kGrad, int kResidual, int kVector, int kTeam, int kHeld>
+__global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_norm_backward_kernel(const BackwardArgs a) {
     constexpr int kOut = kResidual != kNone ? kResidual : kGrad;
     constexpr int kRows = kBatch<kHeld, 2>;
-    __shared__ uint32_t shared[2][kBlock / 32];
-    const Team<kTeam> team{shared};
+    constexpr int kSide = kTogether<kTeam, kRows>;
+    __shared__ uint32_t shared[kSide][kMaxWarps];
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kBlock / kTeam * kRows) + threadIdx.x / kTeam;
-    auto row_at = [&](const int b) { return first + b * (kBlock / kTeam); };
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kTeamBlock<kTeam> / kTeam * kRows) + threadIdx.x / kTeam;
+    auto row_at = [&](const int b) { return first + b * (kTeamBlock<kTeam> / kTeam); };
     Held<kGrad, kVector, kTeam, kHeld> grad[kRows];
     HeldCodes<kVector, kTeam, kHeld> codes[kRows];
     Held<kOut, kVector, kTeam, kHeld> r[kRows];
@@ -536,39 +568,42 @@ __global__ void __launch_bounds__(kBlock) fz_norm_backward_kernel(const Backward
         rstds[b] = __ldg(a.rstd + row);
     }
     #pragma unroll
-    for (int b = 0; b < kRows; b++) {
-        const int64_t row = row_at(b);
-        if (row >= a.n) return;
-        float g[kHeld], y[kHeld];
-        float dot = 0.0f;
+    for (int of = 0; of < kRows; of += kSide) {
+        float mean[kSide] = {};
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            g[i] = grad[b].value(i);
-            y[i] = codes[b].value(i) * scales[b];
-            dot = fmaf(g[i], y[i], dot);
+        for (int b = 0; b < kSide; b++) {
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) mean[b] = fmaf(grad[of + b].value(i), codes[of + b].value(i) * scales[of + b], mean[b]);
         }
-        const float mean = team.sum(dot, b % 2) * a.one_over_d;
+        Team<kTeam, kSide>::sum(mean, shared);
         #pragma unroll
-        for (int i = 0; i < kHeld; i++) {
-            g[i] = rstds[b] * fmaf(-y[i], mean, g[i]);
-            if constexpr (kResidual != kNone) g[i] += r[b].value(i);
+        for (int b = 0; b < kSide; b++) {
+            const int64_t row = row_at(of + b);
+            if (row >= a.n) return;
+            mean[b] *= a.one_over_d;
+            float g[kHeld];
+            #pragma unroll
+            for (int i = 0; i < kHeld; i++) {
+                g[i] = rstds[of + b] * fmaf(-(codes[of + b].value(i) * scales[of + b]), mean[b], grad[of + b].value(i));
+                if constexpr (kResidual != kNone) g[i] += r[of + b].value(i);
+            }
+            store_row<kOut, kVector, kTeam>(row_of<kOut>(a.grad_x, row, a.grad_x_stride), d, t, g);
         }
-        store_row<kOut, kVector, kTeam>(row_of<kOut>(a.grad_x, row, a.grad_x_stride), d, t, g);
     }
 }
 
 template <int kGrad, int kResidual>
 __global__ void __launch_bounds__(kBlock) fz_long_norm_backward_kernel(const BackwardArgs a) {
     constexpr int kOut = kResidual != kNone ? kResidual : kGrad;
-    __shared__ uint32_t shared[1][kBlock / 32];
-    const Team<kBlock> team{shared};
+    __shared__ uint32_t shared[1][kMaxWarps];
     const int64_t row = blockIdx.x;
     const void* grad = row_of<kGrad>(a.grad, row, a.grad_stride);
     const int8_t* codes = a.codes + row * a.codes_stride;
     const float scale = __ldg(a.scales + row), rstd = __ldg(a.rstd + row);
-    float dot = 0.0f;
-    for (int64_t j = threadIdx.x; j < a.d; j += kBlock) dot = fmaf(load_one<kGrad>(grad, j), static_cast<float>(codes[j]) * scale, dot);
-    const float mean = team.sum(dot, 0) * a.one_over_d;
+    float dot[1] = {0.0f};
+    for (int64_t j = threadIdx.x; j < a.d; j += kBlock) dot[0] = fmaf(load_one<kGrad>(grad, j), static_cast<float>(codes[j]) * scale, dot[0]);
+    Team<kBlock, 1>::sum(dot, shared);
+    const float mean = dot[0] * a.one_over_d;
     void* out = row_of<kOut>(a.grad_x, row, a.grad_x_stride);
     for (int64_t j = threadIdx.x; j < a.d; j += kBlock) {
         float g = rstd * fmaf(-static_cast<float>(codes[j]) * scale, mean, load_one<kGrad>(grad, j));
@@ -579,8 +614,11 @@ __global__ void __launch_bounds__(kBlock) fz_long_norm_backward_kernel(const Bac
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-bool aligned(const void* p, const int64_t stride, const int size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+// elements per access that the rows of a tensor allow
+int width_of(const void* p, const int64_t stride, const int size) {
+    const uintptr_t address = reinterpret_cast<uintptr_t>(p);
+    if (address % 16 == 0 && stride * size % 16 == 0) return 8;
+    return address % (2 * size) == 0 && stride % 2 == 0 ? 2 : 1;
 }
 bool valid_type(const int type) { return type == ZF_FLOAT32 || type == ZF_BFLOAT16; }
 int size_of(const int type) { return type == ZF_FLOAT32 ? 4 : 2; }
@@ -593,45 +631,64 @@ bool valid_rows(const void* p, const int type, const int64_t stride, const int64
 
 constexpr int64_t kMaxRows = (int64_t{1} << 31) - 1;  // one block per row at the most
 
-// the team that holds rows of d elements: team threads of which each holds `held` elements
-template <typename Launch, typename LaunchLong>
+// the team that holds rows of d elements, of which each thread holds `held`. With wide accesses a few threads that hold
+// more are faster (a reduction inside a warp needs no barrier; 48,336 x 592 bf16: 41 us in warps of 32 held, 54 in blocks of
+// 128 threads); with narrow ones more threads are (48,335 x 585: 135 against 75 us), as a thread's accesses are many.
+template <int kVector, typename Launch, typename LaunchLong>
 void with_team(const int64_t d, const Launch& launch, const LaunchLong& launch_long) {
     using std::integral_constant;
+    constexpr bool kWide = kVector == 8;
     if (d <= 64) launch(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (d <= 128) launch(integral_constant<int, 16>{}, integral_constant<int, 8>{});
     else if (d <= 256) launch(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else if (d <= 1024) launch(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (d <= 512) launch(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else if (d <= 1024) launch(integral_constant<int, kWide ? 32 : 128>{}, integral_constant<int, kWide ? 32 : 8>{});
+    else if (d <= 2048) launch(integral_constant<int, 256>{}, integral_constant<int, 8>{});
     else if (d <= 4096) launch(integral_constant<int, 256>{}, integral_constant<int, 16>{});
-    else if (d <= 8192) launch(integral_constant<int, 256>{}, integral_constant<int, 32>{});
+    else if (d <= 8192) launch(integral_constant<int, kWide ? 256 : 512>{}, integral_constant<int, kWide ? 32 : 16>{});
     else launch_long();
 }
 
+// elements per access: 8, 2 or 1
+template <typename Launch>
+void with_vector(const int vector, const Launch& launch) {
+    using std::integral_constant;
+    if (vector == 8) launch(integral_constant<int, 8>{});
+    else if (vector == 2) launch(integral_constant<int, 2>{});
+    else launch(integral_constant<int, 1>{});
+}
+
 template <int kX, int kResidual, bool kNorm>
-cudaError_t launch_quantize(const QuantizeArgs& a, const bool vector, cudaStream_t stream) {
-    with_team(
-        a.d,
-        [&](const auto team, const auto held) {
-            constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
-            constexpr int kRows = kBlock / kTeam * kBatch<kHeld, kResidual != kNone ? 2 : 1>;
-            const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
-            if (vector) fz_quantize_kernel<kX, kResidual, kNorm, true, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
-            else fz_quantize_kernel<kX, kResidual, kNorm, false, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
-        },
-        [&] { fz_long_quantize_kernel<kX, kResidual, kNorm><<<static_cast<unsigned>(a.n), kBlock, 0, stream>>>(a); });
+cudaError_t launch_quantize(const QuantizeArgs& a, const int vector, cudaStream_t stream) {
+    with_vector(vector, [&](const auto width) {
+        constexpr int kVector = decltype(width)::value;
+        with_team<kVector>(
+            a.d,
+            [&](const auto team, const auto held) {
+                constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
+                constexpr int kRows = kTeamBlock<kTeam> / kTeam * kBatch<kHeld, kResidual != kNone ? 2 : 1>;
+                const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
+                fz_quantize_kernel<kX, kResidual, kNorm, kVector, kTeam, kHeld><<<blocks, kTeamBlock<kTeam>, 0, stream>>>(a);
+            },
+            [&] { fz_long_quantize_kernel<kX, kResidual, kNorm><<<static_cast<unsigned>(a.n), kBlock, 0, stream>>>(a); });
+    });
     return cudaGetLastError();
 }
 
 template <int kGrad, int kResidual>
-cudaError_t launch_backward(const BackwardArgs& a, const bool vector, cudaStream_t stream) {
-    with_team(
-        a.d,
-        [&](const auto team, const auto held) {
-            constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
-            constexpr int kRows = kBlock / kTeam * kBatch<kHeld, 2>;
-            const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
-            if (vector) fz_norm_backward_kernel<kGrad, kResidual, true, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
-            else fz_norm_backward_kernel<kGrad, kResidual, false, kTeam, kHeld><<<blocks, kBlock, 0, stream>>>(a);
-        },
-        [&] { fz_long_norm_backward_kernel<kGrad, kResidual><<<static_cast<unsigned>(a.n), kBlock, 0, stream>>>(a); });
+cudaError_t launch_backward(const BackwardArgs& a, const int vector, cudaStream_t stream) {
+    with_vector(vector, [&](const auto width) {
+        constexpr int kVector = decltype(width)::value;
+        with_team<kVector>(
+            a.d,
+            [&](const auto team, const auto held) {
+                constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
+                constexpr int kRows = kTeamBlock<kTeam> / kTeam * kBatch<kHeld, 2>;
+                const unsigned blocks = static_cast<unsigned>((a.n + kRows - 1) / kRows);
+                fz_norm_backward_kernel<kGrad, kResidual, kVector, kTeam, kHeld><<<blocks, kTeamBlock<kTeam>, 0, stream>>>(a);
+            },
+            [&] { fz_long_norm_backward_kernel<kGrad, kResidual><<<static_cast<unsigned>(a.n), kBlock, 0, stream>>>(a); });
+    });
     return cudaGetLastError();
 }
 
@@ -644,12 +701,12 @@ cudaError_t launch_restore(const RestoreArgs& a, const bool vector, cudaStream_t
     };
     auto element_wise = [&] { fz_dequantize_flat_kernel<kOut, 1><<<flat(1), kBlock, 0, stream>>>(a); };
     if (vector) {
-        with_team(
+        with_team<8>(
             a.d,
             [&](const auto team, const auto held) {
                 constexpr int kTeam = decltype(team)::value, kHeld = decltype(held)::value;
-                constexpr int kRows = kBlock / kTeam * kBatch<kHeld, 1>;
-                fz_dequantize_kernel<kOut, kTeam, kHeld><<<static_cast<unsigned>((a.n + kRows - 1) / kRows), kBlock, 0, stream>>>(a);
+                constexpr int kRows = kTeamBlock<kTeam> / kTeam * kBatch<kHeld, 1>;
+                fz_dequantize_kernel<kOut, kTeam, kHeld><<<static_cast<unsigned>((a.n + kRows - 1) / kRows), kTeamBlock<kTeam>, 0, stream>>>(a);
             },
             [&] {
                 if (a.out_stride == a.d) fz_dequantize_flat_kernel<kOut, 8><<<flat(8), kBlock, 0, stream>>>(a);
@@ -684,7 +741,7 @@ int zf_quantize_rows(const zf_quantize_rows_args* args, cudaStream_t stream) {
     a.codes = args->codes;
     a.codes_stride = args->codes_stride;
     a.scales = args->scales;
-    const bool vector = aligned(args->x, args->x_stride, size_of(args->x_dtype));
+    const int vector = width_of(args->x, args->x_stride, size_of(args->x_dtype));
     return finish(args->x_dtype == ZF_FLOAT32 ? launch_quantize<kF32, kNone, false>(a, vector, stream) : launch_quantize<kBf16, kNone, false>(a, vector, stream),
                   "quantize_rows");
 }
@@ -698,7 +755,7 @@ int zf_dequantize_rows(const zf_dequantize_rows_args* args, cudaStream_t stream)
     }
     if (!valid_rows(args->out, args->out_dtype, args->out_stride, args->d)) return invalid("dequantize_rows: invalid output");
     const RestoreArgs a{args->codes, args->codes_stride, args->scales, args->n, args->d, args->out, args->out_stride};
-    const bool vector = aligned(args->out, args->out_stride, size_of(args->out_dtype));
+    const bool vector = width_of(args->out, args->out_stride, size_of(args->out_dtype)) == 8;
     return finish(args->out_dtype == ZF_FLOAT32 ? launch_restore<kF32>(a, vector, stream) : launch_restore<kBf16>(a, vector, stream), "dequantize_rows");
 }
 
@@ -720,8 +777,8 @@ int zf_rms_norm_int8(const zf_rms_norm_int8_args* args, cudaStream_t stream) {
                          args->power_of_two != 0, args->codes, args->codes_stride, args->scales, args->sum, args->sum_stride, args->rstd};
     const bool residual = args->residual != nullptr;
     const int size = size_of(args->residual_dtype);
-    const bool vector = aligned(args->x, args->x_stride, size_of(args->x_dtype))
-                        && (!residual || (aligned(args->residual, args->residual_stride, size) && aligned(args->sum, args->sum_stride, size)));
+    int vector = width_of(args->x, args->x_stride, size_of(args->x_dtype));
+    if (residual) vector = std::min({vector, width_of(args->residual, args->residual_stride, size), width_of(args->sum, args->sum_stride, size)});
     cudaError_t error;
     if (args->x_dtype == ZF_FLOAT32) {
         error = !residual ? launch_quantize<kF32, kNone, true>(a, vector, stream)
@@ -752,8 +809,8 @@ int zf_rms_norm_int8_backward(const zf_rms_norm_int8_backward_args* args, cudaSt
     if (!valid_rows(args->grad_x, out_dtype, args->grad_x_stride, args->d)) return invalid("rms_norm_int8_backward: invalid grad_x");
     const BackwardArgs a{args->grad, args->grad_stride, args->codes, args->codes_stride, args->scales, args->rstd, args->grad_residual,
                          args->grad_residual_stride, args->n, args->d, 1.0f / static_cast<float>(args->d), args->grad_x, args->grad_x_stride};
-    const bool vector = aligned(args->grad, args->grad_stride, size_of(args->grad_dtype)) && aligned(args->grad_x, args->grad_x_stride, size_of(out_dtype))
-                        && (!residual || aligned(args->grad_residual, args->grad_residual_stride, size_of(args->grad_residual_dtype)));
+    int vector = std::min(width_of(args->grad, args->grad_stride, size_of(args->grad_dtype)), width_of(args->grad_x, args->grad_x_stride, size_of(out_dtype)));
+    if (residual) vector = std::min(vector, width_of(args->grad_residual, args->grad_residual_stride, size_of(args->grad_residual_dtype)));
     cudaError_t error;
     if (args->grad_dtype == ZF_FLOAT32) {
         error = !residual ? launch_backward<kF32, kNone>(a, vector, stream)
