@@ -22,6 +22,12 @@
 // tile in their order, so that results do not depend on timing. It is launched while the first kernel runs and waits for
 // it.
 //
+// Measured on one B200 (2,097,152 samples, 256 -> 256, with bias): 0.33 ms, 4.9 TB/s of the 6.5 that a copy moves (0.40 ms
+// sustained, when the power cap holds the clock at about 1.5 GHz), against a floor of 0.25 ms for the bytes. A stage takes
+// about 1,100 cycles, 850 of them the MMA thread's (four MMAs run 512) and 220 its share of the additions to the running
+// sum. Ring stages hold gradients and codes until the MMAs are done and values only from the workers to the MMAs: with all
+// three in one slot the copies' latency showed.
+//
 // Bounded waits, pairs and the status as in fz_int8_linear.cu.
 #include "zf_int8.h"
 #include "fz_status.h"
@@ -458,7 +464,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) fz_int8_weight_grad_join_kern
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (live) {
         const float4* from = reinterpret_cast<const float4*>(a.partial) + tile * (a.tile_in / 4) * kTileOut + static_cast<int64_t>(column_word) * kTileOut + row;
-        #pragma unroll 4
+        #pragma unroll 8
         for (int s = kSpread ? warp : 0; s < a.splits; s += kSpread ? kJoinWarps : 1) {
             const float4 v = __ldcs(from + s * a.words);
             sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;

@@ -397,6 +397,30 @@ def test_offsets_past_32_bits(backend):
     assert torch.equal(backend.dequantize_rows(codes, scales)[-3:], backend.dequantize_rows(last[0], last[1]))
 
 
+def test_the_sum_and_the_gradient_in_place(backend):
+    """Through the C ABI: the sum over the residual's own memory, the norm's gradient over the upstream gradient's"""
+    import ctypes
+
+    from zipnerf_b200 import capi
+    lib = capi.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    for n, d in [(37, 256), (5, 99), (3, 3000), (2, 9000)]:
+        x, r = rows(n, d, 1, torch.bfloat16), rows(n, d, 2)
+        wanted = backend.rms_norm_int8(x, r, None, EPS)
+        codes = torch.empty(n, (d + 15) // 16 * 16, device='cuda', dtype=torch.int8)[:, :d]
+        scales, rstd, total = torch.empty_like(wanted[1]), torch.empty_like(wanted[3]), r.clone()
+        args = capi.zf_rms_norm_int8_args(x.data_ptr(), capi.ZF_BFLOAT16, d, total.data_ptr(), capi.ZF_FLOAT32, d, None, n, d, EPS, 0, codes.data_ptr(),
+                                          codes.stride(0), scales.data_ptr(), total.data_ptr(), d, rstd.data_ptr())
+        capi.check(lib.zf_rms_norm_int8(ctypes.byref(args), stream))
+        assert all(torch.equal(a, b) for a, b in zip((codes, scales, total, rstd), wanted))
+        g = rows(n, d, 3)
+        wanted = backend.rms_norm_int8_backward(g, codes, scales, rstd, None)
+        args = capi.zf_rms_norm_int8_backward_args(g.data_ptr(), capi.ZF_FLOAT32, d, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rstd.data_ptr(),
+                                                   None, 0, 0, n, d, g.data_ptr(), d)
+        capi.check(lib.zf_rms_norm_int8_backward(ctypes.byref(args), stream))
+        assert torch.equal(g, wanted)
+
+
 def test_refusals(backend):
     x = rows(4, 32, 1)
     codes, scales = backend.quantize_rows(x)
