@@ -244,7 +244,7 @@ private:
     }
 };
 
-// the same for codes: kVector of them in kWords words
+// the same for codes, kPerWord of them in a word
 template <int kVector, int kTeam, int kHeld>
 struct HeldCodes {
     static constexpr int kPerWord = kVector == 8 ? 4 : kVector;

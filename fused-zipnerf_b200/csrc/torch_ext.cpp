@@ -24,6 +24,7 @@
 
 #include <pybind11/stl.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -671,11 +672,15 @@ at::Tensor empty_codes(const int64_t n, const int64_t d, const at::Device& devic
 
 int8_t* code_ptr(const at::Tensor& codes) { return static_cast<int8_t*>(codes.data_ptr()); }
 
-// the int32 that the tensor-core kernels of a device set to 1 if one of their bounded waits ran out
+// the int32 that the tensor-core kernels of a device set to 1 if one of their bounded waits ran out; made at the device's
+// first use and kept to the process's end
 at::Tensor int8_status(const at::Device& device) {
-    static std::vector<at::Tensor> status(static_cast<size_t>(c10::cuda::device_count()));
-    at::Tensor& t = status.at(static_cast<size_t>(device.index()));
-    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(device));
+    if (!device.is_cuda()) throw std::runtime_error("ZipNeRF: the status belongs to a cuda device");
+    static auto& status = *new std::vector<at::Tensor>(static_cast<size_t>(c10::cuda::device_count()));
+    const int index = device.has_index() ? device.index() : c10::cuda::current_device();
+    if (index < 0 || index >= static_cast<int>(status.size())) throw std::runtime_error("ZipNeRF: no such cuda device");
+    at::Tensor& t = status[static_cast<size_t>(index)];
+    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, static_cast<at::DeviceIndex>(index))));
     return t;
 }
 

@@ -99,6 +99,14 @@ def test_the_binding_refuses_cpu_tensors():
             call()
 
 
+def test_the_status_is_a_cuda_device_s():
+    import ZipNeRFCudaBackend as backend
+    with pytest.raises(RuntimeError, match='ZipNeRF: the status belongs to a cuda device'):
+        backend.int8_status(torch.device('cpu'))
+    with pytest.raises(RuntimeError, match='ZipNeRF: no such cuda device'):
+        backend.int8_status(torch.device('cuda', 63))
+
+
 def test_every_operator_is_reachable_by_name():
     import ZipNeRFCudaBackend
     from ZipNeRFCudaBackend import _C
