@@ -31,6 +31,7 @@
 // Bounded waits, pairs and the status as in fz_int8_linear.cu.
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_grad_words.h"
 #include "fz_launch.h"
 #include "fz_pair.cuh"
 #include "fz_tcgen05.cuh"
@@ -236,12 +237,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
         constexpr int kFetched = kOnGrid ? 1 : kRows / kTeam;
         uint32_t next[kFetched][3] = {};
         const int odd = static_cast<int>((reinterpret_cast<uintptr_t>(a.grad) / 2 + static_cast<uint64_t>(w) * a.grad_stride + out0) & 1);
-        const bool needs[3] = {2 * lane - odd < grad_columns, 2 * (lane + 32) - odd < grad_columns, lane == 31 && 128 - odd < grad_columns};
+        const bool needs[3] = {word_needed(lane, odd, grad_columns), word_needed(lane + 32, odd, grad_columns),
+                               lane == 31 && word_needed(64, odd, grad_columns)};
         auto fetch = [&](const int i) {
             if (i >= stages) return;
             const int64_t row0 = row_of(i);
             const uint16_t* from = a.grad + (row0 + w) * a.grad_stride + out0;
-            if (row0 > 0 && row0 + kRows < a.n) {  // whole words of every row lie in the tensor
+            if (whole_words(row0, kRows, a.n)) {
                 const uint32_t* words = reinterpret_cast<const uint32_t*>(from - odd) + lane;
                 #pragma unroll
                 for (int r = 0; r < kFetched; r++) {
@@ -257,7 +259,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) fz_int8
                 const bool live = row0 + w + kTeam * r < a.n;
                 #pragma unroll
                 for (int j = 0; j < 3; j++) {
-                    const int c = 2 * (j == 2 ? 64 : lane + 32 * j) - odd;  // the word's first column
+                    const int c = word_column(j == 2 ? 64 : lane + 32 * j, odd);
                     const uint32_t lo = live && needs[j] && c >= 0 ? from[c] : 0u, hi = live && needs[j] && c + 1 < grad_columns ? from[c + 1] : 0u;
                     next[r][j] = lo | hi << 16;
                 }
