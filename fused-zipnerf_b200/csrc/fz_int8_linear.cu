@@ -432,7 +432,9 @@ __global__ void __launch_bounds__(kThreads, 1) fz_int8_linear_kernel(const __gri
                     if (lane == 0) {
                         const uint32_t bytes = static_cast<uint32_t>(rows * a.out) * sizeof(Out), whole = bytes & ~15u;
                         uint8_t* to = static_cast<uint8_t*>(a.output) + static_cast<int64_t>(row0) * a.out * sizeof(Out);
-                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_address(staging)), "r"(whole) : "memory");
+                        if (whole > 0) {  // a few rows of a narrow output may be less than the copy's 16 bytes
+                            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_address(staging)), "r"(whole) : "memory");
+                        }
                         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                         // the last rows' last elements
                         for (uint32_t e = whole; e < bytes; e += sizeof(Out)) *reinterpret_cast<Out*>(to + e) = *reinterpret_cast<const Out*>(staging + e);
