@@ -190,8 +190,16 @@ __device__ __forceinline__ int element(const int t, const int i) {
     return i / kVector * (kVector * kTeam) + kVector * t + i % kVector;
 }
 
+// one word of a row. kWritten: of a tensor whose memory may be an output's too (the sum over the residual, a gradient over its
+// upstream gradients), which the non-coherent path must not read.
+template <bool kWritten, typename T>
+__device__ __forceinline__ T load_word(const T* p) {
+    if constexpr (kWritten) return *p;
+    else return __ldg(p);
+}
+
 // a thread's elements of a row as they lie in memory: fetch only loads, value(i) converts. Elements past d are zero.
-template <int kType, int kVector, int kTeam, int kHeld>
+template <int kType, int kVector, int kTeam, int kHeld, bool kWritten>
 struct Held {
     static constexpr int kPerWord = kVector > 1 && kType == kBf16 ? 2 : 1;
     uint32_t words[kHeld / kPerWord];
@@ -205,15 +213,15 @@ struct Held {
             if constexpr (kVector == 8) {
                 #pragma unroll
                 for (int q = 0; q < 2 / kPerWord; q++) {
-                    const uint4 v = j + 8 <= d ? __ldg(reinterpret_cast<const uint4*>(from) + q) : make_uint4(0, 0, 0, 0);
+                    const uint4 v = j + 8 <= d ? load_word<kWritten>(reinterpret_cast<const uint4*>(from) + q) : make_uint4(0, 0, 0, 0);
                     to[4 * q] = v.x, to[4 * q + 1] = v.y, to[4 * q + 2] = v.z, to[4 * q + 3] = v.w;
                 }
             }
             else if constexpr (kVector == 2 && kType == kF32) {
-                const uint2 v = j + 2 <= d ? __ldg(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
+                const uint2 v = j + 2 <= d ? load_word<kWritten>(reinterpret_cast<const uint2*>(from)) : make_uint2(0, 0);
                 to[0] = v.x, to[1] = v.y;
             }
-            else if constexpr (kVector == 2) to[0] = j + 2 <= d ? __ldg(reinterpret_cast<const uint32_t*>(from)) : 0u;
+            else if constexpr (kVector == 2) to[0] = j + 2 <= d ? load_word<kWritten>(reinterpret_cast<const uint32_t*>(from)) : 0u;
             else to[0] = j < d ? bits(row, j) : 0u;
         }
         if (kVector > 1 && d % kVector != 0) {  // the last elements, in the team's thread whose access they do not fill
@@ -239,8 +247,8 @@ struct Held {
 
 private:
     static __device__ __forceinline__ uint32_t bits(const void* row, const int j) {
-        if constexpr (kType == kF32) return __ldg(static_cast<const uint32_t*>(row) + j);
-        else return __ldg(static_cast<const uint16_t*>(row) + j);
+        if constexpr (kType == kF32) return load_word<kWritten>(static_cast<const uint32_t*>(row) + j);
+        else return load_word<kWritten>(static_cast<const uint16_t*>(row) + j);
     }
 };
 
@@ -321,12 +329,14 @@ __global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_quantize_kernel(const Qu
     const int d = static_cast<int>(a.d);
     // a team's rows: the teams of a block side by side, kRows times
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (kTeamBlock<kTeam> / kTeam * kRows) + threadIdx.x / kTeam;
+    if (first >= a.n) return;  // a team without rows: the reductions are a team's own
     auto row_at = [&](const int b) { return first + b * (kTeamBlock<kTeam> / kTeam); };
-    Held<kX, kVector, kTeam, kHeld> x[kRows];
-    Held<kResidual != kNone ? kResidual : kX, kVector, kTeam, kHeld> r[kRows];
+    Held<kX, kVector, kTeam, kHeld, false> x[kRows];
+    Held<kResidual != kNone ? kResidual : kX, kVector, kTeam, kHeld, true> r[kRows];
     #pragma unroll
     for (int b = 0; b < kRows; b++) {
-        const int64_t row = min(row_at(b), a.n - 1);  // rows past the last repeat it and write nothing
+        // rows past the last repeat the team's own first one, which no other team writes, and write nothing
+        const int64_t row = row_at(b) < a.n ? row_at(b) : first;
         x[b].fetch(row_of<kX>(a.x, row, a.x_stride), d, t);
         if constexpr (kResidual != kNone) r[b].fetch(row_of<kResidual>(a.residual, row, a.residual_stride), d, t);
     }
@@ -557,14 +567,16 @@ __global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_norm_backward_kernel(con
     const int t = threadIdx.x % kTeam;
     const int d = static_cast<int>(a.d);
     const int64_t first = static_cast<int64_t>(blockIdx.x) * (kTeamBlock<kTeam> / kTeam * kRows) + threadIdx.x / kTeam;
+    if (first >= a.n) return;  // a team without rows: the reductions are a team's own
     auto row_at = [&](const int b) { return first + b * (kTeamBlock<kTeam> / kTeam); };
-    Held<kGrad, kVector, kTeam, kHeld> grad[kRows];
+    Held<kGrad, kVector, kTeam, kHeld, true> grad[kRows];
     HeldCodes<kVector, kTeam, kHeld> codes[kRows];
-    Held<kOut, kVector, kTeam, kHeld> r[kRows];
+    Held<kOut, kVector, kTeam, kHeld, true> r[kRows];
     float scales[kRows], rstds[kRows];
     #pragma unroll
     for (int b = 0; b < kRows; b++) {
-        const int64_t row = min(row_at(b), a.n - 1);  // rows past the last repeat it and write nothing
+        // rows past the last repeat the team's own first one, which no other team writes, and write nothing
+        const int64_t row = row_at(b) < a.n ? row_at(b) : first;
         grad[b].fetch(row_of<kGrad>(a.grad, row, a.grad_stride), d, t);
         codes[b].fetch(a.codes + row * a.codes_stride, d, t);
         if constexpr (kResidual != kNone) r[b].fetch(row_of<kResidual>(a.grad_residual, row, a.grad_residual_stride), d, t);

@@ -41,3 +41,32 @@ def test_linear_with_a_last_group_of_few_bytes(backend, n, k, o, dtype):  # noqa
     slack = 3 * U * product.abs() + U * wanted.abs() + (BF16 if dtype == torch.bfloat16 else U) * wanted.abs()
     assert ((out.double() - wanted).abs() <= slack * (1 + 1e-3)).all()
     assert backend.int8_status(codes.device).item() == 0
+
+
+@pytest.mark.parametrize('n,d', [(1001, 40), (4133, 256), (3001, 512), (2501, 283), (777, 1000), (501, 4096), (301, 8000), (33, 9001)])
+def test_outputs_over_inputs_with_teams_past_the_last_row(backend, n, d):  # noqa: F811
+    """Through the C ABI, where many teams work at once and the last of them has rows past the end: the sum over the
+    residual, the gradient over either upstream gradient, with the bits of a call into memory of its own"""
+    import ctypes
+
+    from zipnerf_b200 import capi
+    lib = capi.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    for dtype, tag in ((torch.float32, capi.ZF_FLOAT32), (torch.bfloat16, capi.ZF_BFLOAT16)):
+        x, r = rows(n, d, 1, torch.bfloat16), rows(n, d, 2, dtype)
+        wanted = backend.rms_norm_int8(x, r, None, EPS, True)
+        codes = torch.empty(n, (d + 15) // 16 * 16, device='cuda', dtype=torch.int8)[:, :d]
+        scales, rstd, total = torch.empty_like(wanted[1]), torch.empty_like(wanted[3]), r.clone()
+        args = capi.zf_rms_norm_int8_args(x.data_ptr(), capi.ZF_BFLOAT16, d, total.data_ptr(), tag, d, None, n, d, EPS, 1, codes.data_ptr(),
+                                          codes.stride(0), scales.data_ptr(), total.data_ptr(), d, rstd.data_ptr())
+        capi.check(lib.zf_rms_norm_int8(ctypes.byref(args), stream))
+        assert all(torch.equal(a, b) for a, b in zip((codes, scales, total, rstd), wanted))
+        g, gr = rows(n, d, 3, dtype), rows(n, d, 4, dtype)
+        wanted = backend.rms_norm_int8_backward(g, codes, scales, rstd, gr)
+        for over in (0, 1):
+            operands = [g.clone(), gr.clone()]
+            out = operands[over]
+            args = capi.zf_rms_norm_int8_backward_args(operands[0].data_ptr(), tag, d, codes.data_ptr(), codes.stride(0), scales.data_ptr(), rstd.data_ptr(),
+                                                       operands[1].data_ptr(), tag, d, n, d, out.data_ptr(), d)
+            capi.check(lib.zf_rms_norm_int8_backward(ctypes.byref(args), stream))
+            assert torch.equal(out, wanted)
