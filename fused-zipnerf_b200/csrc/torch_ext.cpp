@@ -862,6 +862,9 @@ void int8_weight_grad(const at::Tensor& grad, const at::Tensor& codes, const at:
 }  // namespace
 
 PYBIND11_MODULE(_C, m) {
+    // the defaults below are converted while this module loads, which needs torch's scalar types: also where nobody has
+    // imported torch yet
+    pybind11::module_::import("torch");
     m.attr("grid_max_value") = zf_grid_max_value();
     m.attr("nerf_grid_grad_scale") = zf_nerf_grid_grad_scale();
     m.def("set_rtc_dirs", &set_rtc_dirs);
