@@ -18,6 +18,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -673,14 +674,26 @@ at::Tensor empty_codes(const int64_t n, const int64_t d, const at::Device& devic
 int8_t* code_ptr(const at::Tensor& codes) { return static_cast<int8_t*>(codes.data_ptr()); }
 
 // the int32 that the tensor-core kernels of a device set to 1 if one of their bounded waits ran out; made at the device's
-// first use and kept to the process's end
+// first use and kept to the process's end. It is cleared on a stream of its own before anyone gets it: a fill on the
+// caller's stream would not be ordered before another stream's kernels, and inside a graph capture every replay would
+// repeat it.
 at::Tensor int8_status(const at::Device& device) {
     if (!device.is_cuda()) throw std::runtime_error("ZipNeRF: the status belongs to a cuda device");
     static auto& status = *new std::vector<at::Tensor>(static_cast<size_t>(c10::cuda::device_count()));
     const int index = device.has_index() ? device.index() : c10::cuda::current_device();
     if (index < 0 || index >= static_cast<int>(status.size())) throw std::runtime_error("ZipNeRF: no such cuda device");
     at::Tensor& t = status[static_cast<size_t>(index)];
-    if (!t.defined()) t = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(at::Device(at::kCUDA, static_cast<at::DeviceIndex>(index))));
+    if (!t.defined()) {
+        const at::Device of(at::kCUDA, static_cast<at::DeviceIndex>(index));
+        const c10::cuda::CUDAGuard guard(of);
+        // allocations and waits outside a capture are allowed while one is under way
+        const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+        const c10::cuda::CUDAStream stream = c10::cuda::getStreamFromPool(false, of.index());
+        const c10::cuda::CUDAStreamGuard on(stream);
+        const at::Tensor cleared = at::zeros({1}, at::TensorOptions().dtype(at::kInt).device(of));
+        stream.synchronize();
+        t = cleared;
+    }
     return t;
 }
 
