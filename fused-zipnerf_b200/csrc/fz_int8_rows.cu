@@ -11,8 +11,8 @@
 // 6.0 to 7.0 TB/s against the 6.5 that a copy moves; the norm issues an instruction in 77 % of the cycles, so it is close to
 // that bound as well. Odd widths (1 element per access) reach 2 to 4 TB/s, bound by their many narrow accesses.
 //
-// Compiled without fast math: the quotients are IEEE ones and subnormal inputs are kept, so that the codes are those of
-// the definition.
+// Compiled without fast math: the scales are IEEE quotients and subnormal inputs are kept; the codes are those of the fp32
+// quotients x / scale (to_codes_of).
 #include "zf_int8.h"
 #include "fz_status.h"
 
@@ -122,28 +122,46 @@ struct Team {
 
 __device__ __forceinline__ uint32_t magnitude_bits(const float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+// what turns the values of a row into codes: the scale's reciprocal as the sum of two floats, the second zero for powers of two
+struct Reciprocal {
+    float high, low;
+};
+
 // the scale of a row from the largest magnitude's bits (which order like the magnitudes, infinities and NaN above every
-// finite value), and the factor that turns values into codes: the scale's reciprocal, exact for powers of two, else
-// within an ulp
-__device__ __forceinline__ float row_scale(const uint32_t largest, const bool power_of_two, float& to_codes) {
-    to_codes = 0.0f;
+// finite value), and its reciprocal
+__device__ __forceinline__ float row_scale(const uint32_t largest, const bool power_of_two, Reciprocal& to_codes) {
+    to_codes = {0.0f, 0.0f};
     if (largest == 0) return 0.0f;
     if (largest >= kInfinityBits) return __uint_as_float(0x7FFFFFFFu);
     if (power_of_two) {
         // largest / 127 = m 2^e / 127 with 127 = 1.984375 x 2^6: at most 2^(e - 6) exactly when m is at most 1.984375
         const int exponent = max(static_cast<int>((largest + 0x00020000u - 1u) >> 23) - 6, 1);
-        to_codes = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
+        to_codes.high = __uint_as_float(static_cast<uint32_t>(254 - exponent) << 23);
         return __uint_as_float(static_cast<uint32_t>(exponent) << 23);
     }
     const float scale = fmaxf(__fdiv_rn(__uint_as_float(largest), kLargestCode), kSmallestScale);
-    asm("rcp.approx.f32 %0, %1;" : "=f"(to_codes) : "f"(scale));
+    to_codes.high = __frcp_rn(scale);
+    // 1 - high scale is a float, so it is exact; 1 / scale = high / (1 - error)
+    const float error = fmaf(-to_codes.high, scale, 1.0f);
+    to_codes.low = to_codes.high * fmaf(error, error, error);
     return scale;
 }
 
-// x / scale to the nearest integer, ties to even, in the low byte: the sum with 1.5 x 2^23 leaves the integer in the low
-// bits of the significand, and the product is not rounded before. The product with the reciprocal is within 2 ulp of the
-// quotient: at most 127 (1 + 2^-21), so it cannot round to 128.
-__device__ __forceinline__ uint32_t to_code(const float v, const float to_codes) { return __float_as_uint(fmaf(v, to_codes, 12582912.0f)); }
+// two values as codes, x / scale (the fp32 quotient) to the nearest integer, ties to even, in the low bytes of the words: the
+// sum with 1.5 x 2^23 leaves the integer in the low bits of the significand. The high part alone gives products up to 2 ulp
+// from the quotient, and rows meet half steps often (in bf16 every x of half the largest magnitude is one). With both parts
+// the product is the quotient but where that lies within 2^-46 of a rounding boundary, and its code is the quotient's for every
+// significand of a scale, at every half step and the floats around it (all 7.5e9 compared on the host), for scales
+// below 2^102, where the low part is a normal number. At most 127 (1 + 2^-23), so it cannot round to 128. Division itself,
+// for values near a half step alone, made quantizing 2,097,152 x 256 bf16 415 us instead of 300 (the high part alone: 290).
+__device__ __forceinline__ void to_codes_of(const float x, const float y, const Reciprocal& to_codes, uint32_t& x_code, uint32_t& y_code) {
+    asm("{\n.reg .b64 v, high, low, p;\n"
+        "mov.b64 v, {%2, %3};\nmov.b64 high, {%4, %4};\nmov.b64 low, {%5, %5};\n"
+        "mul.rn.f32x2 p, v, low;\nfma.rn.f32x2 p, v, high, p;\n"
+        "mov.b64 v, {0f4B400000, 0f4B400000};\nadd.rn.f32x2 p, p, v;\nmov.b64 {%0, %1}, p;\n}\n"
+        : "=r"(x_code), "=r"(y_code)
+        : "f"(x), "f"(y), "f"(to_codes.high), "f"(to_codes.low));
+}
 
 // the low bytes of four words
 __device__ __forceinline__ uint32_t pack_codes(const uint32_t a, const uint32_t b, const uint32_t c, const uint32_t d) {
@@ -392,28 +410,33 @@ __global__ void __launch_bounds__(kTeamBlock<kTeam>) fz_quantize_kernel(const Qu
             const int64_t row = row_at(of + b);
             if (row >= a.n) return;
             if (overflow[b]) largest[b] = kInfinityBits;
-            float to_codes;
+            Reciprocal to_codes;
             const float scale = row_scale(largest[b], a.power_of_two, to_codes);
             if (t == 0) a.scales[row] = scale;
             const uint32_t keep = largest[b] < kInfinityBits ? 0xFFFFFFFFu : 0u;  // the codes of a row that is not finite are zero
             int8_t* codes = a.codes + row * a.codes_stride;
+            constexpr int kPairs = kVector > 1 ? kVector : 2;
+            uint32_t pairs[kPairs];
             #pragma unroll
             for (int i = 0; i < kHeld; i += kVector) {
                 const int j = element<kVector, kTeam>(t, i);
-                uint32_t words[kVector];
-                #pragma unroll
-                for (int e = 0; e < kVector; e++) words[e] = to_code(v[b][i + e], to_codes) & keep;
+                if (i % kPairs == 0) {
+                    #pragma unroll
+                    for (int e = 0; e < kPairs; e += 2) to_codes_of(v[b][i + e], v[b][i + e + 1], to_codes, pairs[e], pairs[e + 1]);
+                }
+                const uint32_t* words = pairs + i % kPairs;
                 if (j + kVector <= d) {
                     if constexpr (kVector == 8) {
-                        *reinterpret_cast<uint2*>(codes + j) = make_uint2(pack_codes(words[0], words[1], words[2], words[3]), pack_codes(words[4], words[5], words[6], words[7]));
+                        *reinterpret_cast<uint2*>(codes + j) =
+                            make_uint2(pack_codes(words[0], words[1], words[2], words[3]) & keep, pack_codes(words[4], words[5], words[6], words[7]) & keep);
                     }
-                    else if constexpr (kVector == 2) *reinterpret_cast<uint16_t*>(codes + j) = static_cast<uint16_t>(__byte_perm(words[0], words[1], 0x0040u));
-                    else codes[j] = static_cast<int8_t>(words[0]);
+                    else if constexpr (kVector == 2) *reinterpret_cast<uint16_t*>(codes + j) = static_cast<uint16_t>(__byte_perm(words[0], words[1], 0x0040u) & keep);
+                    else codes[j] = static_cast<int8_t>(words[0] & keep);
                 }
                 else {
                     #pragma unroll
                     for (int e = 0; e + 1 < kVector; e++) {
-                        if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e]);
+                        if (j + e < d) codes[j + e] = static_cast<int8_t>(words[e] & keep);
                     }
                 }
             }
@@ -455,7 +478,7 @@ __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const Quantize
     for (int64_t j = threadIdx.x; j < a.d; j += kBlock) largest[0] = max(largest[0], magnitude_bits(scaled(value(j), j)));
     Row::max(largest, shared[1]);
     if (overflow) largest[0] = kInfinityBits;
-    float to_codes;
+    Reciprocal to_codes;
     const float scale = row_scale(largest[0], a.power_of_two, to_codes);
     if (threadIdx.x == 0) a.scales[row] = scale;
     const bool finite = largest[0] < kInfinityBits;
@@ -464,7 +487,9 @@ __global__ void __launch_bounds__(kBlock) fz_long_quantize_kernel(const Quantize
         const float v = value(j);
         // each thread reads an element of the residual for the last time before it writes the same element of the sum
         if constexpr (kResidual != kNone) store_one<kResidual>(row_of<kResidual>(a.sum, row, a.sum_stride), j, v);
-        codes[j] = static_cast<int8_t>(finite ? to_code(scaled(v, j), to_codes) : 0u);
+        uint32_t code, unused;
+        to_codes_of(scaled(v, j), 0.0f, to_codes, code, unused);
+        codes[j] = static_cast<int8_t>(finite ? code : 0u);
     }
 }
 

@@ -10,7 +10,8 @@
  *
  * Quantization of a row x with a = max |x_j|:
  *   scale = a / 127, or with power_of_two the smallest power of two that is no less; never below 2^-126;
- *   codes = x / scale rounded to nearest, ties to even.
+ *   codes = x / scale, the fp32 quotient, rounded to nearest, ties to even (for scales of 2^102 and more a value within 2^-18
+ *   of a half step may take either of its neighbours).
  *   a = 0: scale 0 and codes 0. A NaN or an infinity anywhere in the row: scale NaN and codes 0, so that every value read
  *   back from the row is NaN.
  * With a power-of-two scale every value codes * scale is a bf16 number (8 significant bits), so tensor-core operands

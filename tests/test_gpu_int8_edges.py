@@ -70,3 +70,19 @@ def test_outputs_over_inputs_with_teams_past_the_last_row(backend, n, d):  # noq
                                                        operands[1].data_ptr(), tag, d, n, d, out.data_ptr(), d)
             capi.check(lib.zf_rms_norm_int8_backward(ctypes.byref(args), stream))
             assert torch.equal(out, wanted)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('n,d', [(20000, 256), (4000, 1000), (4001, 283), (3000, 98), (500, 4097), (301, 5002), (100, 9001)])
+def test_codes_are_the_rounded_quotients(backend, n, d, dtype):  # noqa: F811
+    """Without power-of-two scales too: codes = the fp32 quotient x / scale to the nearest integer, ties to even. Rows hold
+    many values at and beside a half step, where another rounding of the quotient gives the neighbouring code."""
+    x = torch.randn(n, d, device='cuda', generator=generator(d))
+    half_steps = torch.randint(-127, 127, (n, d), device='cuda', generator=generator(n)).float() + 0.5
+    largest = x.abs().amax(1, keepdim=True)
+    x[:, ::2] = (half_steps * (largest / 127))[:, ::2].clamp(-largest, largest)
+    x = x.to(dtype)
+    codes, scales = backend.quantize_rows(x, False)
+    # a 64-bit quotient of fp32 numbers rounded to fp32 is the fp32 quotient: 53 >= 2 * 24 + 2 bits
+    assert torch.equal(scales, (x.double().abs().amax(1) / 127).float())
+    assert torch.equal(codes.float(), torch.round((x.double() / scales.double()[:, None]).float()))
