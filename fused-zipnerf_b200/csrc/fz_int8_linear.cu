@@ -666,6 +666,7 @@ int zf_int8_linear(const zf_int8_linear_args* args, cudaStream_t stream) {
         return invalid("int8_linear: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
     if (args->scales == nullptr || args->weight_scales == nullptr || args->status == nullptr) return invalid("int8_linear: scales and status must be given");
+    if (!zf::aligned_as<float>(args->scales, args->weight_scales, args->bias, args->status)) return invalid("int8_linear: misaligned scales, bias or status");
     const int size = args->output_dtype == ZF_FLOAT32 ? 4 : 2;
     if ((args->output_dtype != ZF_FLOAT32 && args->output_dtype != ZF_BFLOAT16) || args->output == nullptr || args->output_stride < args->out
         || reinterpret_cast<uintptr_t>(args->output) % size != 0) {

@@ -15,6 +15,7 @@
 // quotients x / scale (to_codes_of).
 #include "zf_int8.h"
 #include "fz_status.h"
+#include "fz_launch.h"
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -773,6 +774,7 @@ int zf_quantize_rows(const zf_quantize_rows_args* args, cudaStream_t stream) {
     if (!valid_codes(args->codes, args->codes_stride, args->d) || args->scales == nullptr) {
         return invalid("quantize_rows: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
+    if (!zf::aligned_as<float>(args->scales)) return invalid("quantize_rows: misaligned scales");
     QuantizeArgs a{};
     a.x = args->x;
     a.x_stride = args->x_stride;
@@ -794,6 +796,7 @@ int zf_dequantize_rows(const zf_dequantize_rows_args* args, cudaStream_t stream)
     if (!valid_codes(args->codes, args->codes_stride, args->d) || args->scales == nullptr) {
         return invalid("dequantize_rows: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
+    if (!zf::aligned_as<float>(args->scales)) return invalid("dequantize_rows: misaligned scales");
     if (!valid_rows(args->out, args->out_dtype, args->out_stride, args->d)) return invalid("dequantize_rows: invalid output");
     const RestoreArgs a{args->codes, args->codes_stride, args->scales, args->n, args->d, args->out, args->out_stride};
     const bool vector = width_of(args->out, args->out_stride, size_of(args->out_dtype)) == 8;
@@ -814,6 +817,7 @@ int zf_rms_norm_int8(const zf_rms_norm_int8_args* args, cudaStream_t stream) {
     if (!valid_codes(args->codes, args->codes_stride, args->d) || args->scales == nullptr) {
         return invalid("rms_norm_int8: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
+    if (!zf::aligned_as<float>(args->scales, args->weight, args->rstd)) return invalid("rms_norm_int8: misaligned scales, weight or rstd");
     const QuantizeArgs a{args->x, args->x_stride, args->residual, args->residual_stride, args->weight, args->n, args->d, 1.0f / static_cast<float>(args->d), args->eps,
                          args->power_of_two != 0, args->codes, args->codes_stride, args->scales, args->sum, args->sum_stride, args->rstd};
     const bool residual = args->residual != nullptr;
@@ -846,6 +850,7 @@ int zf_rms_norm_int8_backward(const zf_rms_norm_int8_backward_args* args, cudaSt
     if (!valid_codes(args->codes, args->codes_stride, args->d) || args->scales == nullptr || args->rstd == nullptr) {
         return invalid("rms_norm_int8_backward: codes must be 16-byte aligned with a row stride that is a multiple of 16");
     }
+    if (!zf::aligned_as<float>(args->scales, args->rstd)) return invalid("rms_norm_int8_backward: misaligned scales or rstd");
     const int out_dtype = residual ? args->grad_residual_dtype : args->grad_dtype;
     if (!valid_rows(args->grad_x, out_dtype, args->grad_x_stride, args->d)) return invalid("rms_norm_int8_backward: invalid grad_x");
     const BackwardArgs a{args->grad, args->grad_stride, args->codes, args->codes_stride, args->scales, args->rstd, args->grad_residual,

@@ -581,6 +581,9 @@ int zf_int8_weight_grad(const zf_int8_weight_grad_args* args, cudaStream_t strea
     if (args->grad == nullptr || args->grad_stride < args->out || args->scales == nullptr || args->grad_weight == nullptr || args->status == nullptr) {
         return invalid("int8_weight_grad: invalid grad, scales, grad_weight or status");
     }
+    if (!zf::aligned_as<uint16_t>(args->grad) || !zf::aligned_as<float>(args->scales, args->grad_weight, args->grad_bias, args->status)) {
+        return invalid("int8_weight_grad: misaligned grad, scales, grad_weight, grad_bias or status");
+    }
     if (args->workspace == nullptr || reinterpret_cast<uintptr_t>(args->workspace) % 16 != 0
         || args->workspace_bytes < zf_int8_weight_grad_workspace_size(args->n, args->in, args->out)) {
         return invalid("int8_weight_grad: workspace too small");

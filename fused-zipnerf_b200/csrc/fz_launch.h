@@ -1,11 +1,19 @@
-// fz_launch.h -- host-side launch helpers shared by the 8-bit operators: what a launch asks of a device, asked once.
+// fz_launch.h -- host-side launch helpers shared by the 8-bit operators: what a launch asks of a device, asked once; the
+// alignment of what it is given.
 #pragma once
 
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstdint>
 
 namespace zf {
+
+// every pointer lies on a multiple of T's size (null does too): another address would fault on the device
+template <typename T, typename... P>
+bool aligned_as(const P*... pointers) {
+    return ((reinterpret_cast<uintptr_t>(pointers) % sizeof(T) == 0) && ...);
+}
 
 constexpr int kMaxDevices = 64;
 

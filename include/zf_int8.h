@@ -18,8 +18,8 @@
  * made from it carry no second rounding; the step is between 1 and 2 times a / 127.
  *
  * Conventions as zf_featurize.h: device pointers and sizes, work is only enqueued on the given stream, a failed call
- * returns its status and leaves the message in zf_last_error(). Strides are in elements. n = 0 is valid and launches
- * nothing.
+ * returns its status and leaves the message in zf_last_error(). Strides are in elements; a pointer off its element's
+ * alignment is refused. n = 0 is valid and launches nothing.
  */
 #ifndef ZF_INT8_H
 #define ZF_INT8_H
