@@ -86,3 +86,18 @@ def test_codes_are_the_rounded_quotients(backend, n, d, dtype):  # noqa: F811
     # a 64-bit quotient of fp32 numbers rounded to fp32 is the fp32 quotient: 53 >= 2 * 24 + 2 bits
     assert torch.equal(scales, (x.double().abs().amax(1) / 127).float())
     assert torch.equal(codes.float(), torch.round((x.double() / scales.double()[:, None]).float()))
+
+
+@pytest.mark.parametrize('n', [20, 150])
+def test_the_largest_sums_on_the_tensor_cores(backend, n):  # noqa: F811
+    """Codes -128 and 127 over 131,071 inputs in tiles of one CTA and of a pair: sums of up to 2^31 - 16,384, exact"""
+    k = 131071
+    codes = torch.full((n, k + 1), -128, device='cuda', dtype=torch.int8)[:, :k]
+    codes[1::3] = 127
+    w_codes = torch.full((33, k + 1), -128, device='cuda', dtype=torch.int8)[:, :k]
+    w_codes[::2] = 127
+    scales, w_scales = torch.ones(n, device='cuda'), torch.ones(33, device='cuda')
+    out = backend.int8_linear(codes, scales, w_codes, w_scales, None, False, torch.float32)
+    exact = codes[:, :1].double() * w_codes[:, 0].double() * k  # every input has the same codes
+    assert torch.equal(out, exact.float())
+    assert backend.int8_status(codes.device).item() == 0
