@@ -7,8 +7,8 @@
 // kBatch rows at a time and issues all of their loads, of every operand, before it touches the first value: a conversion
 // behind a load waits for it, and with one load at a time per thread the memory's latency bound these kernels. Rows longer than the widest team holds are walked three times by a block (fz_long_* kernels).
 //
-// Measured on one B200, 2,097,152 x 256 bf16: quantize 0.27 ms, restore 0.24 ms, add + norm 0.56 ms, norm backward 0.54 ms,
-// 6.0 to 7.0 TB/s against the 6.5 that a copy moves; the norm issues an instruction in 77 % of the cycles, so it is close to
+// Measured on one B200, 2,097,152 x 256 bf16: quantize 0.27 ms, restore 0.24 ms, add + norm 0.57 ms, norm backward 0.52 ms,
+// 6.0 to 7.2 TB/s against the 6.5 that a copy moves; the norm issues an instruction in 74 % of the cycles, so it is close to
 // that bound as well. Odd widths (1 element per access) reach 2 to 4 TB/s, bound by their many narrow accesses.
 //
 // Compiled without fast math: the scales are IEEE quotients and subnormal inputs are kept; the codes are those of the fp32

@@ -22,11 +22,13 @@
 // tile in their order, so that results do not depend on timing. It is launched while the first kernel runs and waits for
 // it.
 //
-// Measured on one B200 (2,097,152 samples, 256 -> 256, with bias): 0.33 ms, 4.9 TB/s of the 6.5 that a copy moves (0.40 ms
-// sustained, when the power cap holds the clock at about 1.5 GHz), against a floor of 0.25 ms for the bytes. A stage takes
-// about 1,100 cycles, 850 of them the MMA thread's (four MMAs run 512) and 220 its share of the additions to the running
-// sum. Ring stages hold gradients and codes until the MMAs are done and values only from the workers to the MMAs: with all
-// three in one slot the copies' latency showed.
+// Measured on one B200 (2,097,152 samples, 256 -> 256, with bias): 0.33 ms, 4.9 TB/s of the 6.5 that a copy moves (0.38 to
+// 0.40 ms sustained, when the power cap holds the clock at about 1.5 GHz), against a floor of 0.25 ms for the bytes. The join
+// takes 0.01 ms of it. A pair's 443 stages take 1,180 cycles each (the difference of two row counts) and the launch, the first
+// stages and the sums' way out another 23,000: 546,000 cycles, 0.32 ms at the 1.7 GHz that the kernel runs at. Of a stage's
+// cycles 850 are the MMA thread's (four MMAs run 512) and 220 its share of the additions to the running sum; the other 110
+// are not accounted for. Ring stages hold gradients and codes until the MMAs are done and values only from the workers to the
+// MMAs: with all three in one slot the copies' latency showed.
 //
 // Bounded waits, pairs and the status as in fz_int8_linear.cu.
 #include "zf_int8.h"

@@ -15,7 +15,7 @@ Training keeps one code per activation, the very operands of the forward's produ
 instead of the 16 of a bf16 record. The backward passes gradients straight through the rounding to codes and reads the
 codes: weight gradients by `int8_weight_grad`, the norms by `rms_norm_int8_backward`. The ReLU masks come from running the
 up layer again on its codes, which gives the forward's bits. Data gradients are plain bf16 products with the weights'
-restored values.
+restored values. Forward and backward only enqueue: a caller reads `int8_status` where it synchronises, as the fit below does.
 
     python -m zipnerf_b200.trunk --samples 65536 --steps 100       # fits random features to a fixed random decoder
 """
