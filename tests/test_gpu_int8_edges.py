@@ -101,3 +101,33 @@ def test_the_largest_sums_on_the_tensor_cores(backend, n):  # noqa: F811
     exact = codes[:, :1].double() * w_codes[:, 0].double() * k  # every input has the same codes
     assert torch.equal(out, exact.float())
     assert backend.int8_status(codes.device).item() == 0
+
+
+def test_operators_in_a_captured_graph(backend):  # noqa: F811
+    """A forward and backward captured once and replayed on other inputs: the bits of plain calls, the weight gradient's
+    early-launched join among them"""
+    n, d, o = 3000, 256, 131
+    x, g = rows(n, d, 1, torch.bfloat16), rows(n, o, 2, torch.bfloat16)
+    w_codes, w_scales = code_rows(o, d, 3, power_of_two=False)
+    grad_weight, grad_bias = torch.zeros(o, d, device='cuda'), torch.zeros(o, device='cuda')
+
+    def step():
+        codes, scales, total, rstd = backend.rms_norm_int8(x, x, None, EPS, True)
+        out = backend.int8_linear(codes, scales, w_codes, w_scales, None, True)
+        grad_weight.zero_()
+        grad_bias.zero_()
+        backend.int8_weight_grad(g, codes, scales, grad_weight, grad_bias)
+        back = backend.rms_norm_int8_backward(total, codes, scales, rstd, x)
+        return [codes, scales, total, rstd, out, back, grad_weight, grad_bias]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for seed in (4, 5):
+        x.copy_(rows(n, d, seed, torch.bfloat16))
+        g.copy_(rows(n, o, seed + 2, torch.bfloat16))
+        graph.replay()
+        replayed = [t.clone() for t in captured]
+        for got, wanted in zip(replayed, step()):
+            assert torch.equal(got, wanted)
+    del graph
