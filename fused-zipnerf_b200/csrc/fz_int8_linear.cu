@@ -19,9 +19,9 @@
 // bulk copy writes them, whose start is on the grid again (32 rows). Any other layout is written 32 columns at a time.
 //
 // Measured on one B200: 2,097,152 x 256 -> 256 bf16 with bias and ReLU 0.27 ms, 6.0 TB/s of the 6.5 that a copy moves
-// (floor 0.25 ms); 8,192 x 4,096 -> 4,096 0.108 ms, 2.5 PFLOP/s, or 0.121 ms sustained under the power cap; the tensor pipe
+// (floor 0.25 ms); 8,192 x 4,096 -> 4,096 0.099 ms, 2.8 PFLOP/s, or 0.120 ms sustained under the power cap; the tensor pipe
 // is busy 64 % of the time there, and longer ring stages (two K-blocks per commit) measured the same. Up to 16 rows take
-// fz_int8_linear_few_kernel, whose bound is the weights' bytes and the launch: 1 row 1,024 -> 1,024 2.2 us against 7.5 in
+// fz_int8_linear_few_kernel, whose bound is the weights' bytes and the launch: 1 row 1,024 -> 1,024 2.0 us against 7.5 in
 // tiles, 16 rows 4,096 -> 4,096 11.1 against 17.1.
 //
 // Every wait is bounded: a wait that runs out raises the CTA's abort flag, which ends every role's loop (the other CTA of
